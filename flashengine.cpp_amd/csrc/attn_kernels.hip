@@ -82,25 +82,6 @@ constexpr int dec_units() {
   return FEATTN_DECODE_UNITS;
 }
 
-
-__device__ __forceinline__ DecodeItem ldc_ditem(const DecodeItem* items, int i) {
-  const int32_t* p = reinterpret_cast<const int32_t*>(items + uniform(i));
-  return DecodeItem{ldc(p, 0), ldc(p, 1), ldc(p, 2), ldc(p, 3), ldc(p, 4), ldc(p, 5), ldc(p, 6), ldc(p, 7)};
-}
-
-__device__ __forceinline__ ShareStart ldc_share(const ShareStart* shares, int i) {
-  typedef const __attribute__((address_space(4))) i32x16* const_i32x16p;
-  const i32x16 v = *(const_i32x16p)(shares + uniform(i));
-  ShareStart r;
-  r.it_begin = v[0];
-  r.it_end = v[1];
-  r.first = DecodeItem{v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9]};
-  r.pg0 = v[10];
-  r.pg1 = v[11];
-  r.n_short = v[12];
-  return r;
-}
-
 // NCB: 16-column blocks per item (1 or 2: up to 32 (query row, head)
 // columns, e.g. 8 verify rows with 4 heads per kv head).  Four blocks would
 // need more than the 256 registers of two wavefronts per SIMD.

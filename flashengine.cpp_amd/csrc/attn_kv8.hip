@@ -1,0 +1,1038 @@
+// Paged attention over the 8-bit KV cache (kv8.hpp) for gfx950: the work lists,
+// split-KV partials and merge of the 16-bit kernels, other K/V data movement.
+//
+// The products run on the 16-bit MFMA with the queries' type: the scaled
+// converter turns four codes of one lane into two operand registers, exactly
+// (a code has four significand bits and the scale is a power of two), so that
+// results are those of a 16-bit cache that holds the same values.
+//
+//  * attn_decode_kv8_kernel: a wavefront's share of the decode stream as in
+//    attn_decode_kernel, 32 tokens (two scale blocks) a step.
+//  * attn_short_kv8_kernel: short decode batches.
+//  * attn_tile_kv8_kernel: 64-token tiles shared by four wavefronts.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "attn_types.hpp"
+#include "device_util.hpp"
+#include "kernel_util.hpp"
+#include "kv8.hpp"
+
+namespace feattn {
+
+int decode_wg_waves(int hkv);
+
+// Rows of codes in LDS are 128 bytes, eight 16-byte chunks; chunk c of row t
+// sits at position c ^ swz(t), which spreads every operand read below over
+// all banks, whether the hardware takes 16 lanes (128 bytes) or 32 at a time.
+__device__ __forceinline__ int swz_k(int t) { return ((t >> 1) & 3) | ((((t >> 3) ^ t) & 1) << 2); }
+__device__ __forceinline__ int swz_v(int t) {
+  return ((t >> 1) & 1) | (((t >> 4) & 1) << 1) | ((((t >> 2) ^ t) & 1) << 2);
+}
+
+// V^T operand of a 32-token step: lane 16 J + L of the read for dim block db
+// points at 8 bytes (dims 16 db + 8 m ..) of row k's token, L = 2 k + m: tokens
+// 4 J + k of the first 16 (k < 4) and 4 J + k - 4 of the second, the tokens
+// that the lane's own S^T values belong to.
+__device__ __forceinline__ void v_operand_addr(int J, int L, uint32_t (&v_lds)[8]) {
+  const int k = L >> 1, m = L & 1;
+  const int t = k < 4 ? 4 * J + k : 16 + 4 * J + k - 4;
+#pragma unroll
+  for (int db = 0; db < 8; ++db) v_lds[db] = (uint32_t)(128 * t + 16 * (db ^ swz_v(t)) + 8 * m);
+}
+
+// ===========================================================================
+// Decode
+// ===========================================================================
+// A wavefront owns a ring of U units in LDS, one stream of units per share:
+// per item its Q (16 columns x 256 bytes), then K and V of every 32 tokens
+// (4 KB of codes each).  A unit is five copies, four of 1 KB and one for its
+// scales (the two blocks' K or V scale; for a Q unit a filler, so that the
+// counts of copies in flight stay a multiple of five).
+//
+// Lane = 16*J + L.  Per 32 tokens:
+//   S^T = K Q^T: A = K rows (lane: token L, dims 16 (J + 4 s) .. +15 with one
+//                ds_read_b128 of codes, two k-steps), B = Q^T (the same dims);
+//                C: lane holds tokens 4J+r of column L.
+//   O^T += V^T P^T: A = V^T (v_operand_addr), B = the lane's own S^T values.
+constexpr int kKv8Unit = 4096;
+constexpr int kKv8Slot = kKv8Unit + 256;  // with the scales
+
+#ifndef FEATTN_KV8_UNITS
+#define FEATTN_KV8_UNITS 3
+#endif
+template <int WAVES>
+constexpr int kv8_units() {
+  static_assert(FEATTN_KV8_UNITS * WAVES * kKv8Slot <= kLdsBytes, "decode ring exceeds LDS");
+  return FEATTN_KV8_UNITS;
+}
+
+// ---- short-context items (see attn_short.hpp for the 16-bit form)
+constexpr int kShort8Wave = 16384;  // a wavefront's LDS: 64 tokens of V codes, then its 32 x 128 fp32 results
+template <int WAVES>
+constexpr size_t short8_lds() {
+  return (size_t)WAVES * kShort8Wave + (size_t)WAVES * kDecodeCols * 2 * sizeof(float);
+}
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+
+// K and V scale of a scale block, by a scalar load.
+__device__ __forceinline__ f32x2 ldc_scales(const float* scales, size_t at) {
+  typedef const __attribute__((address_space(4))) f32x2* cp;
+  return *(cp)(scales + 2 * at);
+}
+
+template <bool BF16, int WAVES, int NCB, bool GRID2>
+__device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, int n_items, uint8_t* dsm) {
+  const int lane = threadIdx.x & 63;
+  const int J = lane >> 4;
+  const int L = lane & 15;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int G = a.group;
+  const int row_bytes = a.hkv * kHeadDim;
+  const uint32_t lbase = (uint32_t)(uintptr_t)dsm;
+  const uint32_t vst = lbase + (uint32_t)(wave * kShort8Wave);
+  const uint32_t mlbase = lbase + (uint32_t)(WAVES * kShort8Wave);
+  typedef __attribute__((address_space(3))) float lds_f32;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+
+  const uint32_t k_goff = (uint32_t)(L * row_bytes + 16 * J);
+  uint32_t v_goff[4];  // 8 rows each: blocks 2 i (0, 1) and 2 i + 1 (2, 3) of a 32-token step
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int t = 8 * r + (lane >> 3);
+    v_goff[r] = (uint32_t)((t & 15) * row_bytes + 16 * ((lane & 7) ^ swz_v(t)));
+  }
+  uint32_t v_lds[8];
+  v_operand_addr(J, L, v_lds);
+
+  for (int it = GRID2 ? 0 : blockIdx.x; it < n_items; it += gridDim.x) {
+    const int ri = GRID2 ? (int)blockIdx.y : uniform(it / a.hkv);
+    const int kvh = GRID2 ? (int)blockIdx.x : uniform(it) - ri * a.hkv;
+    const ShortItem* rec = a.shorts + ri;
+    typedef const __attribute__((address_space(4))) i32x8* c_i32x8;
+    typedef const __attribute__((address_space(4))) i32x4* c_i32x4;
+    const i32x8 h = *(c_i32x8)rec;
+    const i32x4 first = *(c_i32x4)(rec->block + 4 * wave);
+    const int q0 = h[0], nq = h[1], vis = h[2], t0 = h[3], t1 = h[4], part = h[5], page_off = h[6];
+    const int ncols = nq * G;
+    const int nblk = (t1 - t0 + 15) >> 4;
+    const int nbw = (nblk + WAVES - 1) / WAVES;     // blocks per wavefront
+    const int nact = (nblk + nbw - 1) / nbw;        // wavefronts with blocks
+    const int b0 = wave * nbw;
+    const int nb = min(nblk, b0 + nbw) - b0;        // this wavefront's blocks (<= 0: none)
+    const int wt0 = t0 + 16 * b0;
+    const int wt1 = min(t1, wt0 + 16 * nb);
+
+    float m[NCB], lsum[NCB];
+    f32x4 o[8][NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      m[cb] = kNegInf;
+      lsum[cb] = 0.f;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    if (nb > 0) {
+      const char* khead = reinterpret_cast<const char*>(a.kc) + (size_t)kvh * kHeadDim;
+      const char* vhead = reinterpret_cast<const char*>(a.vc) + (size_t)kvh * kHeadDim;
+      size_t blk[4];   // scale blocks of the cache
+      f32x2 sc8[4];   // their scales
+      u32x4 kf[4][2];
+      // Blocks past the wavefront's last are read as its last one: every
+      // address is one of the item's, and what they hold is masked.
+      auto locate = [&](int tok, int i) {
+        const int t = min(tok + 16 * i, wt0 + 16 * (nb - 1));
+        const int pg = ldc(a.pages, page_off + (t >> a.page_shift));
+        return ((size_t)pg << (a.page_shift - 4)) + (size_t)((t & ((1 << a.page_shift) - 1)) >> 4);
+      };
+      auto load_k = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            kf[i][s] = *reinterpret_cast<const u32x4*>(khead + blk[i] * (size_t)(16 * row_bytes) + k_goff + 64 * s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc8[i] = ldc_scales(a.scales, blk[i] * (size_t)a.hkv + (size_t)kvh);
+      };
+      auto copy_v = [&](int live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < live) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              lds_dma16(vhead + blk[i] * (size_t)(16 * row_bytes), v_goff[2 * (i & 1) + r],
+                        vst + (uint32_t)(2048 * i + 1024 * r));
+          }
+      };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) blk[i] = (size_t)(uint32_t)first[i];
+      u32x4 qf[NCB][4];
+      int lim[NCB];
+      int lq = lane;
+      asm volatile("" : "+v"(lq));  // (what is derived from the lane alone is not to be held through the item loop)
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int n = 16 * cb + (lq & 15);
+        const bool ok = n < ncols;
+        const int nn = ok ? n : 0;
+        const int r = nn / G;
+        lim[cb] = ok ? min(causal ? vis + r : t1 - 1, wt1 - 1) : -1;
+        const uint16_t* qp = a.q + ((size_t)(q0 + r) * a.hq + kvh * G + (nn - r * G)) * kHeadDim + 16 * (lq >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) qf[cb][k] = ld16(qp + 64 * (k >> 1) + 8 * (k & 1));
+      }
+      load_k();
+      copy_v(nb);
+
+      for (int tok = wt0; tok < wt1; tok += 64) {
+        const int live = min(4, (wt1 - tok + 15) >> 4);
+        wait_vmem<0>();
+        f32x2 sv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sv[i] = sc8[i];
+        f32x4 sc[4][NCB];
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) {
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (tb < live) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const u32x4 w = kf[tb][k >> 1];
+              const u32x4 ka = kv8_decode8<BF16>(w[2 * (k & 1)], w[2 * (k & 1) + 1], sv[tb][0], sv[tb][0]);
+#pragma unroll
+              for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = mfma16<BF16>(ka, qf[cb][k], sc[tb][cb]);
+            }
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const bool more = tok + 64 < wt1;
+        if (more) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) blk[i] = locate(tok + 64, i);
+          load_k();  // under the softmax
+        }
+
+        u32x4 pf[2][NCB];
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+          float mx = kNegInf;
+#pragma unroll
+          for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
+              mx = fmaxf(mx, sc[tb][cb][r]);
+            }
+          mx = max_x32(max_x16(mx));
+          const float mt = mx * a.scale_log2;
+          const bool up = mt > m[cb] + 8.f;  // lazy reference maximum, as in the tile kernel
+          const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
+          if (up) m[cb] = mt;
+          const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+          float x[4][4];
+          float ps = 0.f;
+#pragma unroll
+          for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m_use));
+              ps += x[tb][r];
+            }
+          lsum[cb] = lsum[cb] * alpha + ps;
+          if (__builtin_amdgcn_ballot_w64(up) != 0) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
+          }
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+            pf[ks][cb] = u32x4{pack2<BF16>(x[2 * ks][0], x[2 * ks][1]), pack2<BF16>(x[2 * ks][2], x[2 * ks][3]),
+                               pack2<BF16>(x[2 * ks + 1][0], x[2 * ks + 1][1]),
+                               pack2<BF16>(x[2 * ks + 1][2], x[2 * ks + 1][3])};
+        }
+
+        __builtin_amdgcn_sched_barrier(0);
+        // V rows past the last token, up to the 32-token step they end in,
+        // hold stale cache or LDS contents: zero (0 * stale must stay 0).
+        const int valid = wt1 - tok;
+        const int rows = live > 2 ? 64 : 32;
+        if (valid < rows) {
+          for (int q = 8 * valid + lane; q < 8 * rows; q += 64) lds_zero16(vst + 16 * q);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+          if (ks == 0 || live > 2) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+              const u32x2 w = lds_read_tr8(vst + v_lds[db] + ks * 4096);
+              const u32x4 vf = kv8_decode8<BF16>(w[0], w[1], sv[2 * ks][1], sv[2 * ks + 1][1]);
+#pragma unroll
+              for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[ks][cb], o[db][cb]);
+            }
+          }
+        if (more) {
+          wait_lds();  // the reads of this step's V are complete
+          copy_v((wt1 - tok - 64 + 15) >> 4);
+        }
+      }
+      // fp32 results and statistics to LDS: row = column, 16-byte chunk c
+      // (dims 4 c ..) at chunk position c ^ L.
+      wait_lds();
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      const int Lo = ln & 15, Jo = ln >> 4;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const float ls = sum_x32(sum_x16(lsum[cb]));
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+          *(lds_f32x4*)(uintptr_t)(vst + (uint32_t)(512 * (16 * cb + Lo) + 16 * ((4 * db + Jo) ^ Lo))) = o[db][cb];
+        if (Jo == 0) {
+          const uint32_t ml = mlbase + (uint32_t)(8 * (wave * kDecodeCols + 16 * cb + Lo));
+          *(lds_f32*)(uintptr_t)ml = m[cb];
+          *(lds_f32*)(uintptr_t)(ml + 4) = ls;
+        }
+      }
+    }
+    __syncthreads();
+
+    // Combine: a 32-lane half per column, 4 dims per lane.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int c = ln & 31;
+    for (int n = 2 * wave + (ln >> 5); n < 16 * NCB; n += 2 * WAVES) {
+      if (n >= ncols) break;
+      float mw[WAVES], lw[WAVES];
+      float top = kNegInf;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        mw[w] = kNegInf;
+        lw[w] = 0.f;
+        if (w < nact) {
+          const uint32_t ml = mlbase + (uint32_t)(8 * (w * kDecodeCols + n));
+          mw[w] = *(lds_f32*)(uintptr_t)ml;
+          lw[w] = *(lds_f32*)(uintptr_t)(ml + 4);
+        }
+        top = fmaxf(top, mw[w]);
+      }
+      const float base = top == kNegInf ? 0.f : top;
+      float ls = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        if (w < nact) {
+          const float wt = fast_exp2(mw[w] - base);
+          ls += lw[w] * wt;
+          acc += *(lds_f32x4*)(uintptr_t)(lbase + (uint32_t)(w * kShort8Wave + 512 * n + 16 * (c ^ (n & 15)))) * wt;
+        }
+      const float inv = ls > 0.f ? 1.f / ls : 0.f;
+      const float l2 = ls > 0.f ? top + __log2f(ls) : kNegInf;
+      const int r = n / G, head = kvh * G + (n - r * G);
+      const u32x2 v = {pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
+      if (part < 0) {
+        const size_t oi = (size_t)(q0 + r) * a.hq + head;
+        *reinterpret_cast<u32x2*>(a.out + oi * kHeadDim + 4 * c) = v;
+        if (a.lse != nullptr && c == 0) a.lse[oi] = l2 * kLn2;
+      } else {
+        const size_t oi = (size_t)(part + r) * a.hq + head;
+        *reinterpret_cast<u32x2*>(a.part_o + oi * kHeadDim + 4 * c) = v;
+        if (c == 0) a.part_lse[oi] = l2;
+      }
+    }
+    if constexpr (GRID2) break;
+    if (it + (int)gridDim.x < n_items) __syncthreads();  // the regions are the next item's V
+  }
+}
+
+template <bool BF16, int WAVES, int NCB>
+__global__ __launch_bounds__(64 * WAVES, 2) void attn_short_kv8_kernel(AttnArgs a, int causal) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t dsm[];
+  short_items_kv8<BF16, WAVES, NCB, true>(a, causal, 1, dsm);
+}
+
+// NCB: 16-column blocks per item.  ANY: a graph plan's launch, whose later
+// prepares may plan the batch as short-context items.
+template <bool BF16, int WAVES, int NCB, bool ANY>
+__global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kernel(AttnArgs a, int causal) {
+  constexpr int U = kv8_units<WAVES>();
+  static_assert(U >= 2, "the ring must hold one K/V pair");
+  extern __shared__ __attribute__((aligned(16))) uint8_t dsm[];
+  const int lane = threadIdx.x & 63;
+  const int J = lane >> 4;
+  const int L = lane & 15;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int G = a.group;
+  const int pshift = a.page_shift;
+  const int pmask = (1 << pshift) - 1;
+  const uint32_t ring = (uint32_t)(uintptr_t)dsm + (uint32_t)(wave * U * kKv8Slot);
+
+  const int slot = blockIdx.x * WAVES + wave;
+  const int kvh = slot % a.hkv;
+  const int share = slot / a.hkv;
+  if (!ANY && share >= a.n_share_cap) return;
+  const ShareStart rec = ldc_share(a.shares, ANY ? min(share, a.n_share_cap - 1) : share);
+  if constexpr (ANY) {
+    if constexpr (WAVES >= kShortMinWaves) {
+      if (rec.n_short > 0) {
+        short_items_kv8<BF16, WAVES, NCB, false>(a, causal, rec.n_short, dsm);
+        return;
+      }
+    }
+    if (share >= a.n_share_cap) return;
+  }
+  const int it_begin = rec.it_begin;
+  const int it_end = rec.it_end;
+  if (it_begin >= it_end) return;
+
+  // Copy instruction r of a unit of codes, lane i: row 8 r + i / 8 of its 32,
+  // chunk position i % 8.
+  const int row_bytes = a.hkv * kHeadDim;
+  uint32_t k_goff[2], v_goff[4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int t = 8 * r + (lane >> 3);
+    k_goff[r] = (uint32_t)(t * row_bytes + 16 * ((lane & 7) ^ swz_k(t)));
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int t = 8 * r + (lane >> 3);
+    v_goff[r] = (uint32_t)((t & 15) * row_bytes + 16 * ((lane & 7) ^ swz_v(t)));
+  }
+  // K operand: token L, chunk J + 4 s; Q operand for k-step 2 s + h: column L,
+  // the 16-byte chunk of dims 16 (J + 4 s) + 8 h.
+  uint32_t k_lds[2], q_lds[4], v_lds[8];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) k_lds[s] = (uint32_t)(128 * L + 16 * ((J + 4 * s) ^ swz_k(L)));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) q_lds[k] = (uint32_t)(256 * L + 16 * ((2 * (J + 4 * (k >> 1)) + (k & 1)) ^ L));
+  v_operand_addr(J, L, v_lds);
+
+  const size_t head_off = (size_t)kvh * kHeadDim;
+  auto page_id = [&](const DecodeItem& d, int tok) { return ldc(a.pages, d.page_off + (tok >> pshift)); };
+  auto block_of = [&](int tok, int pg) {
+    return ((size_t)pg << (pshift - 4)) + (size_t)((tok & pmask) >> 4);
+  };
+  auto block_addr = [&](const void* cache, size_t blk) {
+    return reinterpret_cast<const char*>(cache) + head_off + blk * (size_t)(16 * row_bytes);
+  };
+
+  // ---- copy side: the next unit of the share's stream --------------------
+  // kind 0 = Q of item c_it, 1 = K / 2 = V of the 32 tokens at c_tok.  The
+  // following item (nw) and the next K unit's page ids are requested one item
+  // / one unit before they are needed.  A unit whose tokens end in its first
+  // block copies that one twice (what it brings is masked).
+  int c_it = it_begin;
+  DecodeItem cw = rec.first;
+  DecodeItem nw = cw;
+  if (c_it + 1 < it_end) nw = ldc_ditem(a.ditems, c_it + 1);
+  int c_kind = 0;
+  int c_qb = 0;
+  int c_tok = cw.t0;
+  int pg0 = rec.pg0;
+  int pg1 = cw.t0 + 16 < cw.t1 ? rec.pg1 : rec.pg0;
+  size_t blk0 = 0, blk1 = 0;
+  bool c_live = true;
+  int issued = 0;
+  int c_slot = 0;
+
+  auto issue_codes = [&](const void* cache, const uint32_t (&goff)[4], int side, uint32_t dst) {
+    const char* b0 = block_addr(cache, blk0);
+    const char* b1 = block_addr(cache, blk1);
+    lds_dma16<true>(b0, goff[0], dst);
+    lds_dma16<true>(b0, goff[1], dst + 1024);
+    lds_dma16<true>(b1, goff[2], dst + 2048);
+    lds_dma16<true>(b1, goff[3], dst + 3072);
+    const size_t at = (lane & 1) ? blk1 : blk0;
+    lds_dma4(a.scales + 2 * (at * (size_t)a.hkv + (size_t)kvh) + side, dst + kKv8Unit);
+  };
+  auto issue_one = [&]() {
+    const uint32_t dst = ring + (uint32_t)(c_slot * kKv8Slot);
+    if (c_kind == 0) {
+      const int nc = cw.nq * G;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = 4 * r + J;
+        const int col = 16 * c_qb + n;
+        const int nn = col < nc ? col : 0;  // columns past the item repeat column 0
+        const int row = cw.q0 + nn / G;
+        const int head = kvh * G + nn % G;
+        lds_dma16(a.q + ((size_t)row * a.hq + head) * kHeadDim + 8 * (L ^ n), dst + 1024 * r);
+      }
+      lds_dma4(a.q, dst + kKv8Unit);
+      if (++c_qb == NCB) {
+        c_qb = 0;
+        c_kind = 1;
+      }
+    } else if (c_kind == 1) {
+      blk0 = block_of(c_tok, pg0);
+      blk1 = c_tok + 16 < cw.t1 ? block_of(c_tok + 16, pg1) : blk0;
+      const uint32_t kg[4] = {k_goff[0], k_goff[1], k_goff[0], k_goff[1]};
+      issue_codes(a.kc, kg, 0, dst);
+      // pages of the next K unit: later in this item, or the next item's first
+      if (c_tok + 32 < cw.t1) {
+        pg0 = page_id(cw, c_tok + 32);
+        pg1 = page_id(cw, min(c_tok + 48, cw.t1 - 1));
+      } else if (c_it + 1 < it_end) {
+        pg0 = page_id(nw, nw.t0);
+        pg1 = page_id(nw, min(nw.t0 + 16, nw.t1 - 1));
+      }
+      c_kind = 2;
+    } else {
+      issue_codes(a.vc, v_goff, 1, dst);
+      c_tok += 32;
+      c_kind = 1;
+      if (c_tok >= cw.t1) {
+        ++c_it;
+        if (c_it < it_end) {
+          cw = nw;
+          c_tok = cw.t0;
+          c_kind = 0;
+          if (c_it + 1 < it_end) nw = ldc_ditem(a.ditems, c_it + 1);
+        } else {
+          c_live = false;
+        }
+      }
+    }
+    ++issued;
+    c_slot = c_slot + 1 == U ? 0 : c_slot + 1;
+  };
+
+  // ---- compute side --------------------------------------------------------
+  int consumed = 0;
+  int r_slot = 0;
+  auto refill = [&]() {
+    wait_lds();
+    while (c_live && issued - consumed < U) issue_one();
+  };
+  typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
+
+  for (int it = it_begin; it < it_end; ++it) {
+    refill();
+    const DecodeItem w = it == it_begin ? rec.first : ldc_ditem(a.ditems, it);
+    const int t0 = w.t0;
+    const int t1 = w.t1;
+    const int ncols = w.nq * G;
+    bool col_ok[NCB];
+    int crow[NCB], chead[NCB], lim[NCB];  // lim: last visible token of the lane's column
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const int n = 16 * cb + L;
+      col_ok[cb] = n < ncols;
+      crow[cb] = w.q0 + (col_ok[cb] ? n / G : 0);
+      chead[cb] = kvh * G + (col_ok[cb] ? n % G : 0);
+      lim[cb] = -1;
+      if (col_ok[cb]) lim[cb] = min(causal ? w.len - w.nq + (crow[cb] - w.q0) : w.len - 1, t1 - 1);
+    }
+
+    u32x4 qf[NCB][4];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      if (cb > 0) refill();
+      wait_units<U, 5>(issued - consumed - 1);
+      const uint32_t qb = ring + (uint32_t)(r_slot * kKv8Slot);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        qf[cb][k] = lds_read16(qb + q_lds[k]);
+        if (!col_ok[cb]) qf[cb][k] = u32x4{0u, 0u, 0u, 0u};
+      }
+      consumed += 1;
+      r_slot = r_slot + 1 == U ? 0 : r_slot + 1;
+    }
+
+    float m[NCB], lsum[NCB];
+    f32x4 o[8][NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      m[cb] = kNegInf;
+      lsum[cb] = 0.f;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (int tok = t0; tok < t1; tok += 32) {
+      // The workgroup's wavefronts are brought back in step every 64 tokens,
+      // so that each page is requested by all of them at about the same time.
+      if (((tok - t0) & 32) == 0) __builtin_amdgcn_s_barrier();
+      refill();
+      wait_units<U, 5>(issued - consumed - 2);
+      const uint32_t kst = ring + (uint32_t)(r_slot * kKv8Slot);
+      const int v_slot = r_slot + 1 == U ? 0 : r_slot + 1;
+      const uint32_t vst = ring + (uint32_t)(v_slot * kKv8Slot);
+
+      const f32x2 ks = *(lds_f32x2*)(uintptr_t)(kst + kKv8Unit);
+      const f32x2 vs = *(lds_f32x2*)(uintptr_t)(vst + kKv8Unit);
+      f32x4 sc[2][NCB];
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const u32x4 kw = lds_read16(kst + 2048 * tb + k_lds[s]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x4 kf = kv8_decode8<BF16>(kw[2 * h], kw[2 * h + 1], ks[tb], ks[tb]);
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = mfma16<BF16>(kf, qf[cb][2 * s + h], sc[tb][cb]);
+          }
+        }
+      }
+
+      u32x4 pf[NCB];
+      float alpha[NCB];
+      bool any_up = false;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        float x[2][4];
+        float mx = kNegInf;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[tb][r] = tok + 16 * tb + 4 * J + r <= lim[cb] ? sc[tb][cb][r] * a.scale_log2 : kNegInf;
+            mx = fmaxf(mx, x[tb][r]);
+          }
+        mx = max_x32(max_x16(mx));
+        // Lazy reference maximum: raised (with l and o rescaled) only when the
+        // step's maximum exceeds it by more than 8, so p <= 2^8.
+        const bool up = mx > m[cb] + 8.f;
+        alpha[cb] = up ? fast_exp2(m[cb] - mx) : 1.f;
+        if (up) m[cb] = mx;
+        any_up = any_up || up;
+        const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+        float ps = 0.f;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[tb][r] = fast_exp2(x[tb][r] - m_use);
+            ps += x[tb][r];
+          }
+        lsum[cb] = lsum[cb] * alpha[cb] + ps;
+        pf[cb] = u32x4{pack2<BF16>(x[0][0], x[0][1]), pack2<BF16>(x[0][2], x[0][3]), pack2<BF16>(x[1][0], x[1][1]),
+                       pack2<BF16>(x[1][2], x[1][3])};
+      }
+
+      if (t1 - tok < 32) {
+        // Rows past the item end hold stale contents: zero them, so that
+        // 0 * (stale) can never become NaN.  (16-byte chunk q lies in row q / 8.)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int q = lane + 64 * u;
+          if ((q >> 3) >= t1 - tok) lds_zero16(vst + 16 * q);
+        }
+      }
+      if (__builtin_amdgcn_ballot_w64(any_up) != 0) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+          for (int db = 0; db < 8; ++db) o[db][cb] *= alpha[cb];
+      }
+      u32x2 vw[8];
+#pragma unroll
+      for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + v_lds[db]);
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        const u32x4 vf = kv8_decode8<BF16>(vw[db][0], vw[db][1], vs[0], vs[1]);
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[cb], o[db][cb]);
+      }
+      consumed += 2;
+      r_slot = v_slot + 1 == U ? 0 : v_slot + 1;
+    }
+
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const float ls = sum_x32(sum_x16(lsum[cb]));
+      if (col_ok[cb]) {
+        const float inv = ls > 0.f ? 1.f / ls : 0.f;
+        const float l2 = ls > 0.f ? m[cb] + __log2f(ls) : kNegInf;
+        const bool whole = w.part < 0;
+        const size_t oi = whole ? (size_t)crow[cb] * a.hq + chead[cb]
+                                : (size_t)(w.part + (16 * cb + L) / G) * a.hq + chead[cb];
+        uint16_t* op = (whole ? a.out : a.part_o) + oi * kHeadDim + 4 * J;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+          const u32x2 v = {pack2<BF16>(o[db][cb][0] * inv, o[db][cb][1] * inv),
+                           pack2<BF16>(o[db][cb][2] * inv, o[db][cb][3] * inv)};
+          *reinterpret_cast<u32x2*>(op + 16 * db) = v;
+        }
+        if (J == 0) {
+          if (!whole) a.part_lse[oi] = l2;
+          else if (a.lse != nullptr) a.lse[oi] = l2 * kLn2;
+        }
+      }
+    }
+  }
+}
+
+// ===========================================================================
+// Tiles
+// ===========================================================================
+// Four wavefronts share 64-token tiles.  Wavefront w copies the codes of block
+// w of the next tile to a region of its own (4 KB) while the current one is
+// computed; once they have landed it converts them, once for all four, into
+// the 16-bit tile (32 KB: K blocks, then V blocks, 16 tokens x 256 bytes; chunk
+// c of row t at c ^ t in K, c ^ 2t in V), of which there are two.
+constexpr int kTile8Block = 4096;
+constexpr int kTile8Stage = 8 * kTile8Block;
+constexpr int kTile8Raw = 2 * kTile8Stage;           // offset of the wavefronts' code regions
+constexpr int kTile8Lds = kTile8Raw + 4 * 4096;      // 80 KB: two workgroups a compute unit
+
+struct Tile8Lanes {
+  uint32_t goff[2];
+  uint32_t k_lds[4], v_lds[8];
+};
+
+// Requests the codes of this wavefront's block (tokens T + 16 wave ..) of item
+// w's tile at T, and returns its scales; blocks at or past the item end are
+// skipped.
+template <bool STREAM>
+__device__ __forceinline__ f32x2 tile8_copy(const AttnArgs& a, const WorkItem& w, const SeqInfo& s,
+                                             const Tile8Lanes& tl, uint32_t lbase, int wave, int T) {
+  const int tok = T + 16 * wave;
+  if (tok >= w.t1) return f32x2{1.f, 1.f};
+  const int pshift = a.page_shift;
+  const int row_bytes = a.hkv * kHeadDim;
+  const int pg = ldc(a.pages, s.page_off + (tok >> pshift));
+  const size_t blk = ((size_t)pg << (pshift - 4)) + (size_t)((tok & ((1 << pshift) - 1)) >> 4);
+  const size_t off = blk * (size_t)(16 * row_bytes) + (size_t)w.kvh * kHeadDim;
+  const char* kb = reinterpret_cast<const char*>(a.kc) + off;
+  const char* vb = reinterpret_cast<const char*>(a.vc) + off;
+  const uint32_t raw = lbase + (uint32_t)(kTile8Raw + wave * 4096);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) lds_dma16<STREAM>(kb, tl.goff[r], raw + 1024 * r);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) lds_dma16<STREAM>(vb, tl.goff[r], raw + 2048 + 1024 * r);
+  return ldc_scales(a.scales, blk * (size_t)a.hkv + (size_t)w.kvh);
+}
+
+template <bool BF16, bool CAUSAL, int NCB, bool STREAM>
+__device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, const SeqInfo& s, bool has_next,
+                                          const WorkItem& wn, const SeqInfo& sn, const Tile8Lanes& tl, uint32_t lbase,
+                                          int wave, int lane, int stage0, f32x2& scales) {
+  const int J = lane >> 4;
+  const int L = lane & 15;
+  const int G = a.group;
+  const int kvh = w.kvh;
+  const int t0 = w.t0;
+  const int t1 = w.t1;
+  const int ncols = w.nq * G;
+  constexpr int kWcols = 16 * NCB;  // columns per wavefront
+  const bool wave_on = wave * kWcols < ncols;
+
+  int lim[NCB], crow[NCB], chead[NCB];
+  u32x4 qf[NCB][4];
+  int lim_min = 1 << 30;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int n = wave * kWcols + 16 * cb + L;
+    const bool ok = n < ncols;
+    crow[cb] = w.q0 + (ok ? n / G : 0);
+    chead[cb] = kvh * G + (ok ? n % G : 0);
+    lim[cb] = -1;
+    if (ok) lim[cb] = min(CAUSAL ? s.len - s.qlen + (crow[cb] - s.qo) : s.len - 1, t1 - 1);
+    if (ok) lim_min = min(lim_min, lim[cb]);
+    const uint16_t* qp = a.q + ((size_t)crow[cb] * a.hq + chead[cb]) * kHeadDim + 8 * J;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) qf[cb][k] = ld16(qp + 32 * k);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (!ok) qf[cb][k] = u32x4{0u, 0u, 0u, 0u};
+      // (Q has landed past this point: no wait for it inside the tile loop)
+      asm volatile("" : "+v"(qf[cb][k]));
+    }
+  }
+#pragma unroll
+  for (int o_ = 32; o_ >= 1; o_ >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o_, 64));
+
+  float m[NCB], lsum[NCB];
+  f32x4 o[8][NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    m[cb] = kNegInf;
+    lsum[cb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  auto compute = [&](uint32_t st, int T, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    f32x4 sc[4][NCB];
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t kb = st + tl.k_lds[k];
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb) {
+        const u32x4 kf = lds_read16(kb + tb * kTile8Block);
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = mfma16<BF16>(kf, qf[cb][k], sc[tb][cb]);
+      }
+    }
+
+    u32x4 pf[2][NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (MASK) {
+            if (T + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
+          }
+          mx = fmaxf(mx, sc[tb][cb][r]);
+        }
+      mx = max_x32(max_x16(mx));
+      const float mt = mx * a.scale_log2;
+      const bool up = mt > m[cb] + 8.f;  // lazy reference maximum, p <= 2^8
+      const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
+      if (up) m[cb] = mt;
+      const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+      float x[4][4];
+      float ps = 0.f;
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m_use));
+          ps += x[tb][r];
+        }
+      lsum[cb] = lsum[cb] * alpha + ps;
+      if (__builtin_amdgcn_ballot_w64(up) != 0) {
+#pragma unroll
+        for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        pf[ks][cb] = u32x4{pack2<BF16>(x[2 * ks][0], x[2 * ks][1]), pack2<BF16>(x[2 * ks][2], x[2 * ks][3]),
+                           pack2<BF16>(x[2 * ks + 1][0], x[2 * ks + 1][1]),
+                           pack2<BF16>(x[2 * ks + 1][2], x[2 * ks + 1][3])};
+    }
+
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        const uint32_t vb = st + tl.v_lds[db];
+        const u32x2 lo = lds_read_tr16(vb + (4 + 2 * ks) * kTile8Block);
+        const u32x2 hi = lds_read_tr16(vb + (5 + 2 * ks) * kTile8Block);
+        const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[ks][cb], o[db][cb]);
+      }
+    // V^T operand reads three blocks ahead of their MFMAs (LDS latency)
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int i = 0; i < 13; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, NCB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 3 * NCB, 0);
+  };
+
+  int stage = stage0;
+  for (int T = t0; T < t1; T += kTileTokens) {
+    wait_vmem<0>();  // this wavefront's codes have landed
+    const uint32_t st = lbase + (uint32_t)(stage * kTile8Stage);
+    {
+      // Rows at or past the item end become zero in V (0 * stale must stay 0).
+      const uint32_t raw = lbase + (uint32_t)(kTile8Raw + wave * 4096);
+      const int valid = t1 - (T + 16 * wave);
+      const int c = lane & 7;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = 8 * u + (lane >> 3);
+        const u32x4 kw = lds_read16(raw + 16 * lane + 1024 * u);
+        u32x4 vw = lds_read16(raw + 2048 + 16 * lane + 1024 * u);
+        if (t >= valid) vw = u32x4{0u, 0u, 0u, 0u};
+        const uint32_t kd = st + (uint32_t)(wave * kTile8Block + 256 * t);
+        const uint32_t vd = kd + 4 * kTile8Block;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          lds_write16(kd + 16 * (((2 * c + h) ^ t) & 15),
+                      kv8_decode8<BF16>(kw[2 * h], kw[2 * h + 1], scales[0], scales[0]));
+          lds_write16(vd + 16 * (((2 * c + h) ^ (2 * t)) & 15),
+                      kv8_decode8<BF16>(vw[2 * h], vw[2 * h + 1], scales[1], scales[1]));
+        }
+      }
+    }
+    __syncthreads();  // the tile is in LDS, its codes are read, the other tile is free
+    if (T + kTileTokens < t1) scales = tile8_copy<STREAM>(a, w, s, tl, lbase, wave, T + kTileTokens);
+    else if (has_next) scales = tile8_copy<STREAM>(a, wn, sn, tl, lbase, wave, wn.t0);
+    if (wave_on) {
+      if (T + kTileTokens - 1 <= lim_min) compute(st, T, std::false_type{});
+      else compute(st, T, std::true_type{});
+    }
+    stage ^= 1;
+  }
+
+  if (wave_on) {
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const float ln = sum_x32(sum_x16(lsum[cb]));
+      const int n = wave * kWcols + 16 * cb + L;
+      if (n < ncols) {
+        const float inv = ln > 0.f ? 1.f / ln : 0.f;
+        const float l2 = ln > 0.f ? m[cb] + __log2f(ln) : kNegInf;
+        const bool whole = w.part < 0;
+        const size_t oi = whole ? (size_t)crow[cb] * a.hq + chead[cb] : (size_t)(w.part + n / G) * a.hq + chead[cb];
+        uint16_t* op = (whole ? a.out : a.part_o) + oi * kHeadDim + 4 * J;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+          const u32x2 v = {pack2<BF16>(o[db][cb][0] * inv, o[db][cb][1] * inv),
+                           pack2<BF16>(o[db][cb][2] * inv, o[db][cb][3] * inv)};
+          *reinterpret_cast<u32x2*>(op + 16 * db) = v;
+        }
+        if (J == 0) {
+          if (!whole) a.part_lse[oi] = l2;
+          else if (a.lse != nullptr) a.lse[oi] = l2 * kLn2;
+        }
+      }
+    }
+  }
+  return stage;
+}
+
+template <bool BF16, bool CAUSAL, bool STREAM>
+__global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t dsm[];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int J = lane >> 4;
+  const int L = lane & 15;
+  const int n_items = uniform(*a.n_items);
+  const int row_bytes = a.hkv * kHeadDim;
+  const uint32_t lbase = (uint32_t)(uintptr_t)dsm;
+
+  Tile8Lanes tl;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)((8 * r + (lane >> 3)) * row_bytes + 16 * (lane & 7));
+#pragma unroll
+  for (int s = 0; s < 4; ++s) tl.k_lds[s] = (uint32_t)(16 * (16 * L + (((4 * s + J) ^ L) & 15)));
+  {
+    const int k = L >> 2, m = L & 3, t = 4 * J + k;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      const int c = 2 * db + (m >> 1);
+      tl.v_lds[db] = (uint32_t)(16 * (16 * t + ((c ^ (2 * t)) & 15)) + 8 * (m & 1));
+    }
+  }
+
+  int it = ldc(a.tile_off, blockIdx.x);
+  const int end = min(ldc(a.tile_off, blockIdx.x + 1), n_items);
+  if (it >= end) return;
+  WorkItem w = ldc_item(a.items, it);
+  SeqInfo s = ldc_seq(a.seqs, w.seq);
+  f32x2 scales = tile8_copy<STREAM>(a, w, s, tl, lbase, wave, w.t0);
+  int stage = 0;
+  for (;;) {
+    const int nit = it + 1;
+    const bool has_next = nit < end;
+    WorkItem wn = w;
+    SeqInfo sn = s;
+    if (has_next) {
+      wn = ldc_item(a.items, nit);
+      sn = ldc_seq(a.seqs, wn.seq);
+    }
+    if (w.nq * a.group <= 64)
+      stage = tile8_item<BF16, CAUSAL, 1, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
+    else
+      stage = tile8_item<BF16, CAUSAL, 2, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
+    if (!has_next) break;
+    it = nit;
+    w = wn;
+    s = sn;
+  }
+}
+
+// ===========================================================================
+// Launchers
+// ===========================================================================
+enum class Decode8 { Shares, Short, Any };
+
+template <bool BF16, int WAVES, int NCB, Decode8 KIND>
+static hipError_t decode8_launch(const AttnArgs& a, int causal, int grid, hipStream_t st) {
+  void (*fn)(AttnArgs, int);
+  size_t lds = 0;
+  if constexpr (KIND != Decode8::Short) lds = (size_t)WAVES * kv8_units<WAVES>() * kKv8Slot;
+  if constexpr (KIND != Decode8::Shares) lds = std::max(lds, short8_lds<WAVES>());
+  if constexpr (KIND == Decode8::Short) fn = attn_short_kv8_kernel<BF16, WAVES, NCB>;
+  else fn = attn_decode_kv8_kernel<BF16, WAVES, NCB, KIND == Decode8::Any>;
+  static std::atomic<uint64_t> lds_ok{0};
+  const hipError_t e = allow_lds((const void*)fn, lds, lds_ok);
+  if (e != hipSuccess) return e;
+  const dim3 g = KIND == Decode8::Short ? dim3(a.hkv, grid / a.hkv) : dim3(grid);
+  hipLaunchKernelGGL(fn, g, dim3(64 * WAVES), lds, st, a, causal);
+  return hipGetLastError();
+}
+
+template <bool BF16, int WAVES, Decode8 KIND>
+static hipError_t decode8_ncb(const AttnArgs& a, int ncb, int causal, int grid, hipStream_t st) {
+  switch (ncb) {
+    case 1: return decode8_launch<BF16, WAVES, 1, KIND>(a, causal, grid, st);
+    case 2: return decode8_launch<BF16, WAVES, 2, KIND>(a, causal, grid, st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+template <bool BF16, int WAVES>
+static hipError_t decode8_kind(const AttnArgs& a, int ncb, int causal, bool any, int grid, hipStream_t st) {
+  if constexpr (WAVES >= kShortMinWaves) {
+    if (any) return decode8_ncb<BF16, WAVES, Decode8::Any>(a, ncb, causal, grid, st);
+    if (a.n_short > 0) return decode8_ncb<BF16, WAVES, Decode8::Short>(a, ncb, causal, grid, st);
+  } else if (a.n_short > 0) {
+    return hipErrorInvalidValue;
+  }
+  return decode8_ncb<BF16, WAVES, Decode8::Shares>(a, ncb, causal, grid, st);
+}
+
+template <bool BF16>
+static hipError_t decode8_waves(const AttnArgs& a, int waves, int ncb, int causal, bool any, int grid,
+                                hipStream_t st) {
+  switch (waves) {
+    case 8: return decode8_kind<BF16, 8>(a, ncb, causal, any, grid, st);
+    case 4: return decode8_kind<BF16, 4>(a, ncb, causal, any, grid, st);
+    case 2: return decode8_kind<BF16, 2>(a, ncb, causal, any, grid, st);
+    case 1: return decode8_kind<BF16, 1>(a, ncb, causal, any, grid, st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_decode_kv8(const AttnArgs& a, bool bf16, int waves, int ncb, int causal, bool any, int grid,
+                             hipStream_t st) {
+  return bf16 ? decode8_waves<true>(a, waves, ncb, causal, any, grid, st)
+              : decode8_waves<false>(a, waves, ncb, causal, any, grid, st);
+}
+
+template <bool BF16, bool CAUSAL, bool STREAM>
+static hipError_t tile8_launch(const AttnArgs& a, int grid, hipStream_t st) {
+  static std::atomic<uint64_t> lds_ok{0};
+  const hipError_t e = allow_lds((const void*)attn_tile_kv8_kernel<BF16, CAUSAL, STREAM>, kTile8Lds, lds_ok);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((attn_tile_kv8_kernel<BF16, CAUSAL, STREAM>), dim3(grid), dim3(256), kTile8Lds, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, int grid, hipStream_t st) {
+  auto go = [&](auto bf, auto ca) {
+    constexpr bool B = decltype(bf)::value, C = decltype(ca)::value;
+    return stream ? tile8_launch<B, C, true>(a, grid, st) : tile8_launch<B, C, false>(a, grid, st);
+  };
+  using T = std::true_type;
+  using F = std::false_type;
+  if (bf16) return causal ? go(T{}, T{}) : go(T{}, F{});
+  return causal ? go(F{}, T{}) : go(F{}, F{});
+}
+
+}  // namespace feattn

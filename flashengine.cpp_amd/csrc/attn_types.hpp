@@ -131,6 +131,7 @@ struct AttnArgs {
   int group;               // hq / hkv
   int page_shift;          // log2(page)
   float scale_log2;        // log2(e) / sqrt(128)
+  const float* scales;     // 8-bit caches: [16-token block][hkv][2] powers of two (kc, vc then hold e4m3 codes)
 };
 
 struct MergeArgs {

@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <initializer_list>
 #include <new>
 #include <string>
 #include <vector>
@@ -28,6 +29,9 @@ hipError_t launch_decode(const AttnArgs& a, bool bf16, int waves, int ncb, int c
                          hipStream_t st);
 int decode_wg_waves(int hkv);
 hipError_t launch_tile(const AttnArgs& a, bool bf16, bool causal, bool stream, int grid, hipStream_t st);
+hipError_t launch_decode_kv8(const AttnArgs& a, bool bf16, int waves, int ncb, int causal, bool any, int grid,
+                             hipStream_t st);
+hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, int grid, hipStream_t st);
 hipError_t launch_merge(const MergeArgs& a, bool bf16, int grid, hipStream_t st);
 hipError_t launch_stage_copy(void* dst, const void* src, size_t bytes, hipStream_t st);
 hipError_t launch_rope(void* q, void* k, const int64_t* pos, const float* cache, int rows, int hq, int hkv, int dim,
@@ -47,6 +51,17 @@ hipError_t launch_accept(const int64_t* draft, const int64_t* verify, int64_t* o
 hipError_t launch_rope_append(void* q, const void* k, const void* v, void* kc, void* vc, const int64_t* pos,
                               const int64_t* slots, const float* cache, int rows, int hq, int hkv, int dim, bool bf16,
                               int max_pos, int64_t cache_slots, hipStream_t st);
+hipError_t launch_store_kv8(const void* k, const void* v, void* kc, void* vc, float* scales, const int64_t* slots,
+                            int rows, int hkv, bool bf16, int cache_slots, hipStream_t st);
+hipError_t launch_rope_append_kv8(void* q, const void* k, const void* v, void* kc, void* vc, float* scales,
+                                  const int64_t* pos, const int64_t* slots, const float* table, int rows, int hq,
+                                  int hkv, bool bf16, int max_pos, int cache_slots, hipStream_t st);
+hipError_t launch_norm_rope_append_kv8(const void* qkv, int64_t row_stride, const void* qw, const void* kw, float eps,
+                                       void* q_out, void* kc, void* vc, float* scales, const int64_t* pos,
+                                       const int64_t* slots, const float* table, int rows, int hq, int hkv, bool bf16,
+                                       int max_pos, int cache_slots, hipStream_t st);
+hipError_t launch_load_kv8(const void* kc, const void* vc, const float* scales, const int64_t* slots, void* k_out,
+                           void* v_out, int rows, int hkv, bool bf16, int cache_slots, hipStream_t st);
 }  // namespace feattn
 
 using namespace feattn;
@@ -431,8 +446,36 @@ int check_tensors(const void* q, const void* k_cache, const void* v_cache, const
   return FE_OK;
 }
 
-int launch_all(const Launch& L, const void* q, const void* k_cache, const void* v_cache, void* out, float* lse,
-               int causal, hipStream_t st) {
+// The K and V scale of a block and head are read together, 8 bytes.
+int check_scales(const char* what, const float* scales) {
+  if (scales == nullptr) return fail(FE_EINVAL, std::string(what) + ": null pointer");
+  if (reinterpret_cast<uintptr_t>(scales) % 8 != 0)
+    return fail(FE_EINVAL, std::string(what) + ": scales must be 8-byte aligned");
+  return FE_OK;
+}
+
+// What the entry points that write or read an 8-bit cache by slots have in
+// common.
+int check_kv8(const char* what, int rows, int hkv, int dim, int cache_slots) {
+  if (rows < 0 || hkv < 0 || cache_slots < 0) return fail(FE_EINVAL, std::string(what) + ": negative size");
+  if (dim != kHeadDim) return fail(FE_EINVAL, std::string(what) + ": head dim must be 128");
+  if (cache_slots % 16 != 0)
+    return fail(FE_EINVAL, std::string(what) + ": cache_slots must be a multiple of 16 (a scale block)");
+  return FE_OK;
+}
+
+int check_aligned16(const char* what, std::initializer_list<const void*> ptrs) {
+  for (const void* ptr : ptrs) {
+    if (ptr == nullptr) return fail(FE_EINVAL, std::string(what) + ": null pointer");
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return fail(FE_EINVAL, std::string(what) + ": tensors must be 16-byte aligned");
+  }
+  return FE_OK;
+}
+
+// scales != nullptr: the caches hold the 8-bit codes that they scale.
+int launch_all(const Launch& L, const void* q, const void* k_cache, const void* v_cache, const float* scales,
+               void* out, float* lse, int causal, hipStream_t st) {
   const int mode = causal ? 1 : 0;
   const int32_t* hdr = reinterpret_cast<const int32_t*>(L.dev + L.lay.header);
   const uint8_t* heap = L.dev + L.lay.heap;
@@ -453,6 +496,7 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
   while ((1 << shift) < L.sh.page) ++shift;
   a.page_shift = shift;
   a.scale_log2 = 1.4426950408889634f / 11.313708498984761f;  // log2(e) / sqrt(128)
+  a.scales = scales;
   hipError_t e;
   if (L.graph || L.n_decode > 0 || L.n_short > 0) {
     AttnArgs d = a;
@@ -465,7 +509,8 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
     const int grid = L.graph      ? L.grid_decode_cap
                      : d.n_short > 0 ? d.n_short
                                      : std::min(L.grid_decode_cap, (L.n_decode + wv - 1) / wv);
-    e = launch_decode(d, L.bf16, L.decode_wg, L.decode_nc / 16, causal ? 1 : 0, L.graph, std::max(grid, 1), st);
+    e = (scales != nullptr ? launch_decode_kv8 : launch_decode)(d, L.bf16, L.decode_wg, L.decode_nc / 16,
+                                                                causal ? 1 : 0, L.graph, std::max(grid, 1), st);
     if (e != hipSuccess) return hip_fail(e, "decode kernel launch");
   }
   if (L.graph ? L.graph_tile > 0 : L.n_tile[mode] > 0) {
@@ -474,7 +519,8 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
     t.n_items = hdr + (mode ? kHdrTileEnd1 : kHdrTileEnd0);
     t.tile_off = reinterpret_cast<const int32_t*>(L.dev + L.lay.tshare[mode]);
     const int grid = L.graph ? L.grid_tile_cap : L.n_tshare[mode];
-    e = launch_tile(t, L.bf16, causal != 0, L.tile_stream[mode], std::max(grid, 1), st);
+    e = (scales != nullptr ? launch_tile_kv8 : launch_tile)(t, L.bf16, causal != 0, L.tile_stream[mode],
+                                                            std::max(grid, 1), st);
     if (e != hipSuccess) return hip_fail(e, "tile kernel launch");
   }
   if (L.graph || L.n_merge[mode] > 0) {
@@ -591,7 +637,7 @@ int attn_oneshot(uint8_t* arena, size_t bytes, int device, const void* q, const 
   L.part_o = reinterpret_cast<uint16_t*>(arena + o_off);
   L.part_lse = reinterpret_cast<float*>(arena + lse_off);
   record_lists(L, bp, hp, bp.decode_nc);
-  return launch_all(L, q, k_cache, v_cache, out, lse, causal, st);
+  return launch_all(L, q, k_cache, v_cache, nullptr, out, lse, causal, st);
 }
 }  // namespace feattn
 
@@ -754,7 +800,19 @@ int fe_attn_run(fe_attn_plan* p, const void* q, const void* k_cache, const void*
   if (rc != FE_OK) return rc;
   rc = check_stream_device(static_cast<hipStream_t>(stream), p->device);
   if (rc != FE_OK) return rc;
-  return launch_all(p->run, q, k_cache, v_cache, out, lse, causal, static_cast<hipStream_t>(stream));
+  return launch_all(p->run, q, k_cache, v_cache, nullptr, out, lse, causal, static_cast<hipStream_t>(stream));
+}
+
+int fe_attn_run_kv8(fe_attn_plan* p, const void* q, const void* k_cache, const void* v_cache, const float* scales,
+                    void* out, float* lse, int causal, void* stream) {
+  if (p == nullptr) return fail(FE_EINVAL, "plan is null");
+  if (!p->prepared) return fail(FE_EINVAL, "attention called before prepare_plan");
+  int rc = check_tensors(q, k_cache, v_cache, out, lse);
+  if (rc == FE_OK) rc = check_scales("attention (8-bit cache)", scales);
+  if (rc != FE_OK) return rc;
+  rc = check_stream_device(static_cast<hipStream_t>(stream), p->device);
+  if (rc != FE_OK) return rc;
+  return launch_all(p->run, q, k_cache, v_cache, scales, out, lse, causal, static_cast<hipStream_t>(stream));
 }
 
 int fe_attn_plan_lists(const fe_attn_plan* p, int causal, int32_t* counts_out) {
@@ -863,6 +921,76 @@ int fe_norm_rope_append(const void* qkv, int64_t row_stride, const void* q_weigh
                                                slots, cache, rows, hq, hkv, bf16 != 0, max_positions, cache_slots,
                                                static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FE_OK : hip_fail(e, "norm_rope_append kernel launch");
+}
+
+int fe_store_kv8(const void* k, const void* v, void* k_cache, void* v_cache, float* scales, const int64_t* slots,
+                 int rows, int hkv, int dim, int bf16, int cache_slots, void* stream) {
+  const char* what = "store_kv8";
+  int rc = check_kv8(what, rows, hkv, dim, cache_slots);
+  if (rc != FE_OK || rows == 0 || hkv == 0) return rc;
+  rc = check_aligned16(what, {k, v, k_cache, v_cache});
+  if (rc == FE_OK) rc = check_scales(what, scales);
+  if (rc != FE_OK) return rc;
+  if (slots == nullptr) return fail(FE_EINVAL, "store_kv8: null pointer");
+  const hipError_t e = launch_store_kv8(k, v, k_cache, v_cache, scales, slots, rows, hkv, bf16 != 0, cache_slots,
+                                        static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FE_OK : hip_fail(e, "store_kv8 kernel launch");
+}
+
+int fe_rope_append_kv8(void* q, const void* k, const void* v, void* k_cache, void* v_cache, float* scales,
+                       const int64_t* pos, const int64_t* slots, const float* cache, int rows, int hq, int hkv,
+                       int dim, int bf16, int max_positions, int cache_slots, void* stream) {
+  const char* what = "rope_append_kv8";
+  int rc = check_kv8(what, rows, hkv, dim, cache_slots);
+  if (rc != FE_OK) return rc;
+  if (hq < 0) return fail(FE_EINVAL, "rope_append_kv8: negative size");
+  if (rows == 0 || hq + hkv == 0) return FE_OK;
+  if (hq > 0) rc = check_aligned16(what, {q, cache});
+  if (rc == FE_OK && hkv > 0) rc = check_aligned16(what, {k, v, k_cache, v_cache, cache});
+  if (rc == FE_OK && hkv > 0) rc = check_scales(what, scales);
+  if (rc != FE_OK) return rc;
+  if (pos == nullptr || (hkv > 0 && slots == nullptr)) return fail(FE_EINVAL, "rope_append_kv8: null pointer");
+  if (hq > 0 && hkv > 0 && (q == k || q == v)) return fail(FE_EINVAL, "rope_append_kv8: q must not alias k or v");
+  const hipError_t e = launch_rope_append_kv8(q, k, v, k_cache, v_cache, scales, pos, slots, cache, rows, hq, hkv,
+                                              bf16 != 0, max_positions, cache_slots, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FE_OK : hip_fail(e, "rope_append_kv8 kernel launch");
+}
+
+int fe_norm_rope_append_kv8(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, float eps,
+                            void* q_out, void* k_cache, void* v_cache, float* scales, const int64_t* pos,
+                            const int64_t* slots, const float* cache, int rows, int hq, int hkv, int dim, int bf16,
+                            int max_positions, int cache_slots, void* stream) {
+  const char* what = "norm_rope_append_kv8";
+  int rc = check_kv8(what, rows, hkv, dim, cache_slots);
+  if (rc != FE_OK) return rc;
+  if (hq < 0) return fail(FE_EINVAL, "norm_rope_append_kv8: negative size");
+  if (rows == 0 || hq + hkv == 0) return FE_OK;
+  if (row_stride < ((int64_t)hq + 2 * (int64_t)hkv) * dim || row_stride % 8 != 0)
+    return fail(FE_EINVAL, "norm_rope_append_kv8: row_stride must cover hq + 2*hkv heads and be a multiple of 8");
+  rc = check_aligned16(what, {qkv, cache});
+  if (rc == FE_OK && hq > 0) rc = check_aligned16(what, {q_weight, q_out});
+  if (rc == FE_OK && hkv > 0) rc = check_aligned16(what, {k_weight, k_cache, v_cache});
+  if (rc == FE_OK && hkv > 0) rc = check_scales(what, scales);
+  if (rc != FE_OK) return rc;
+  if (pos == nullptr || (hkv > 0 && slots == nullptr)) return fail(FE_EINVAL, "norm_rope_append_kv8: null pointer");
+  const hipError_t e = launch_norm_rope_append_kv8(qkv, row_stride, q_weight, k_weight, eps, q_out, k_cache, v_cache,
+                                                   scales, pos, slots, cache, rows, hq, hkv, bf16 != 0, max_positions,
+                                                   cache_slots, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FE_OK : hip_fail(e, "norm_rope_append_kv8 kernel launch");
+}
+
+int fe_load_kv8(const void* k_cache, const void* v_cache, const float* scales, const int64_t* slots, void* k_out,
+                void* v_out, int rows, int hkv, int dim, int bf16, int cache_slots, void* stream) {
+  const char* what = "load_kv8";
+  int rc = check_kv8(what, rows, hkv, dim, cache_slots);
+  if (rc != FE_OK || rows == 0 || hkv == 0) return rc;
+  rc = check_aligned16(what, {k_cache, v_cache, k_out, v_out});
+  if (rc == FE_OK) rc = check_scales(what, scales);
+  if (rc != FE_OK) return rc;
+  if (slots == nullptr) return fail(FE_EINVAL, "load_kv8: null pointer");
+  const hipError_t e = launch_load_kv8(k_cache, v_cache, scales, slots, k_out, v_out, rows, hkv, bf16 != 0,
+                                       cache_slots, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FE_OK : hip_fail(e, "load_kv8 kernel launch");
 }
 
 int fe_attn_plan_describe(int hq, int hkv, int dim, int page, int max_batch, int max_pages, int blocks,

@@ -41,6 +41,24 @@ __device__ __forceinline__ SeqInfo ldc_seq(const SeqInfo* seqs, int i) {
   return SeqInfo{ldc(p, 0), ldc(p, 1), ldc(p, 2), ldc(p, 3)};
 }
 
+__device__ __forceinline__ DecodeItem ldc_ditem(const DecodeItem* items, int i) {
+  const int32_t* p = reinterpret_cast<const int32_t*>(items + uniform(i));
+  return DecodeItem{ldc(p, 0), ldc(p, 1), ldc(p, 2), ldc(p, 3), ldc(p, 4), ldc(p, 5), ldc(p, 6), ldc(p, 7)};
+}
+
+__device__ __forceinline__ ShareStart ldc_share(const ShareStart* shares, int i) {
+  typedef const __attribute__((address_space(4))) i32x16* const_i32x16p;
+  const i32x16 v = *(const_i32x16p)(shares + uniform(i));
+  ShareStart r;
+  r.it_begin = v[0];
+  r.it_end = v[1];
+  r.first = DecodeItem{v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9]};
+  r.pg0 = v[10];
+  r.pg1 = v[11];
+  r.n_short = v[12];
+  return r;
+}
+
 // 16 bytes per lane from global memory to LDS (lane i's at lds_addr + 16 i).
 // m0 holds the LDS address; the instruction needs a wait state after m0's
 // write.
@@ -90,22 +108,34 @@ __device__ __forceinline__ void lds_dma16(const char* base, uint32_t off, uint32
   }
 }
 
+// 4 bytes per lane (lane i's at lds_addr + 4 i).
+__device__ __forceinline__ void lds_dma4(const void* gaddr, uint32_t lds_addr) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %0, off"
+      :
+      : "v"(gaddr), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
+      : "memory", "m0");
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vmem() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// Waits until at most `n` units (4 copy instructions each) issued after the
+// Waits until at most `n` units (PER copy instructions each) issued after the
 // awaited one are still in flight; n is wave-uniform.  vmcnt holds 6 bits,
-// so n is clamped to 15 (a longer wait, never a shorter one).
-template <int MAXU>
+// so n is clamped to 63 / PER (a longer wait, never a shorter one).
+template <int MAXU, int PER = 4>
 __device__ __forceinline__ void wait_units(int n) {
-  static_for<0, (MAXU < 15 ? MAXU : 15) + 1>([&](auto i) {
+  constexpr int kMost = MAXU < 63 / PER ? MAXU : 63 / PER;
+  static_for<0, kMost + 1>([&](auto i) {
     constexpr int I = decltype(i)::value;
-    if (I == (MAXU < 15 ? MAXU : 15)) {
-      if (n >= I) wait_vmem<4 * I>();
+    if (I == kMost) {
+      if (n >= I) wait_vmem<PER * I>();
     } else if (n == I) {
-      wait_vmem<4 * I>();
+      wait_vmem<PER * I>();
     }
   });
 }
@@ -130,6 +160,20 @@ __device__ __forceinline__ u32x2 lds_read_tr16(uint32_t lds_addr) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)lds_addr);
   return __builtin_bit_cast(u32x2, v);
+}
+
+// The same for bytes: lane 16 J + L, L = 2 k + m, points at 8 bytes of row k
+// and receives column L of its group's 8 rows x 16 columns (lanes m = 0, 1
+// hold columns 8 m .. 8 m + 7).
+__device__ __forceinline__ u32x2 lds_read_tr8(uint32_t lds_addr) {
+  typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uintptr_t)lds_addr));
+}
+
+__device__ __forceinline__ void lds_write16(uint32_t lds_addr, u32x4 v) {
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  *(lds_u32x4*)(uintptr_t)lds_addr = v;
 }
 
 __device__ __forceinline__ u32x4 lds_read16(uint32_t lds_addr) {

@@ -1,0 +1,412 @@
+// Append to the 8-bit paged KV cache (kv8.hpp), with q/k RMSNorm and RoPE on
+// the way, and reading its tokens back as 16-bit rows, for gfx950.
+//
+// Append: for every scale block and kv head that the call writes,
+//   need  = the smallest power of two s with max |x| <= 448 s over the finite
+//           values x that the call puts there
+//   scale = need where the call writes the block's first slot (which starts
+//           the block), else max(old scale, need); where that grows, the codes
+//           already in the block are rescaled
+//   code  = e4m3(x / scale), round to nearest even, rounded once from the fp32
+//           value (normalised, rotated); infinities and NaNs become NaN codes.
+// This file is compiled with -ffp-contract=off (the rope form's queries are
+// bit-identical to fe_rope's).
+#include "kv8.hpp"
+#include "rope_math.hpp"
+
+namespace feattn {
+
+enum class Kv8Form { Store, Rope, NormRope };
+
+struct Kv8Args {
+  const uint16_t* q;  // Rope: rotated in place through q_out (the same tensor)
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_stride, kv_stride;  // elements from row to row
+  const uint16_t* qw;
+  const uint16_t* kw;
+  float eps;
+  uint16_t* q_out;  // [rows][hq][128]
+  uint8_t* kc;
+  uint8_t* vc;
+  uint32_t* scales;
+  const int64_t* pos;
+  const int64_t* slots;
+  const float* table;
+  int rows, hq, hkv, max_pos, cache_slots;
+};
+
+// Sum and maximum over an aligned group of eight lanes, in registers.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_bits(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141;
+
+__device__ __forceinline__ float sum8(float v) {
+  v += __uint_as_float(dpp_bits<kXor1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_bits<kXor2>(__float_as_uint(v)));
+  return v + __uint_as_float(dpp_bits<kHalfMirror>(__float_as_uint(v)));
+}
+__device__ __forceinline__ uint32_t max8(uint32_t v) {
+  v = max(v, dpp_bits<kXor1>(v));
+  v = max(v, dpp_bits<kXor2>(v));
+  return max(v, dpp_bits<kHalfMirror>(v));
+}
+
+// A head's 128 elements lie on eight lanes: lane c holds elements 8c..8c+7 and
+// 64+8c..64+8c+7 (the RoPE pairs), x[0..7] and x[8..15].
+template <bool BF16>
+__device__ __forceinline__ void unpack16(u32x4 lo, u32x4 hi, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = lo_f32<BF16>(lo[i]);
+    x[2 * i + 1] = hi_f32<BF16>(lo[i]);
+    x[8 + 2 * i] = lo_f32<BF16>(hi[i]);
+    x[9 + 2 * i] = hi_f32<BF16>(hi[i]);
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ void normalize16(float (&x)[16], const uint16_t* w, int c, float eps) {
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s = __builtin_fmaf(x[e], x[e], s);
+  const float r = rsqrtf(sum8(s) * (1.f / 128.f) + eps);
+  float g[16];
+  unpack16<BF16>(ldv(w + 8 * c), ldv(w + 64 + 8 * c), g);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = x[e] * r * g[e];
+}
+
+__device__ __forceinline__ void rotate16(float (&x)[16], const float* cs) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float a = x[e], b = x[8 + e], co = cs[e], si = cs[64 + e];
+    x[e] = __fsub_rn(__fmul_rn(a, co), __fmul_rn(b, si));
+    x[8 + e] = __fadd_rn(__fmul_rn(b, co), __fmul_rn(a, si));
+  }
+}
+
+// Query heads, eight lanes each.
+template <bool BF16, Kv8Form FORM>
+__device__ __forceinline__ void kv8_query(const Kv8Args& a, int64_t unit, int c) {
+  if (unit >= (int64_t)a.rows * a.hq) return;  // whole groups of eight lanes
+  const int64_t row = unit / a.hq;
+  const int head = (int)(unit - row * a.hq);
+  const uint16_t* src = a.q + row * a.q_stride + (int64_t)head * 128;
+  uint16_t* dst = a.q_out + unit * 128;
+  const int64_t p = a.pos[row];
+  const bool rot = p >= 0 && p < a.max_pos;
+  const float* cs = a.table + (rot ? p : 0) * 128 + 8 * c;
+  u32x4 lo = ldv(src + 8 * c), hi = ldv(src + 64 + 8 * c);
+  if constexpr (FORM == Kv8Form::Rope) {
+    if (!rot) return;  // in place
+    rotate8<BF16>(lo, hi, cs, cs + 64);
+  } else {
+    float x[16];
+    unpack16<BF16>(lo, hi, x);
+    normalize16<BF16>(x, a.qw, c, a.eps);
+    if (rot) rotate16(x, cs);
+    float l[8], h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      l[e] = x[e];
+      h[e] = x[8 + e];
+    }
+    lo = pack8_rne<BF16>(l);
+    hi = pack8_rne<BF16>(h);
+  }
+  stv(dst + 8 * c, lo);
+  stv(dst + 64 + 8 * c, hi);
+}
+
+// One wavefront takes a window of 16 rows and one (kv head, K or V).  The rows
+// of a call that go to one scale block follow one another; such a run belongs
+// to the window its first row lies in, whose wavefront sees all of its values
+// at once (registers, 8 rows a pass, four passes: a run that starts in the
+// window ends within 32 rows of the window's first) and is the only one to
+// write that block and head: no atomics, and the same bits every time.
+// Lane i (1 <= i <= 32) keeps the books of row r0 - 1 + i.
+template <bool BF16, Kv8Form FORM>
+__device__ __forceinline__ void kv8_window(const Kv8Args& a, int64_t unit) {
+  constexpr int kPasses = 4;
+  const int lane = threadIdx.x & 63;
+  const int c = lane & 7;
+  const int g = lane >> 3;
+  const int64_t heads = 2 * a.hkv;
+  const int64_t win = unit / heads;
+  const int hs = uniform((int)(unit - win * heads));
+  const int side = hs >= a.hkv ? 1 : 0;
+  const int head = side ? hs - a.hkv : hs;
+  const int64_t r0 = win * 16;
+
+  // ---- runs
+  const int64_t row = r0 - 1 + lane;
+  int slot = -1, p = -1;
+  if (lane <= 32 && row >= 0 && row < a.rows) {
+    const int64_t s = a.slots[row];
+    if (s >= 0 && s < a.cache_slots) slot = (int)s;
+    if (FORM != Kv8Form::Store && side == 0) {
+      const int64_t q = a.pos[row];
+      if (q >= 0 && q < a.max_pos) p = (int)q;
+    }
+  }
+  const int block = slot >> 4;  // -1: the row is not stored
+  const int before = __shfl_up(block, 1, 64);
+  // (lane 0: the row before the window, whose run another window owns)
+  const uint64_t heads_of_runs = __builtin_amdgcn_ballot_w64(lane == 0 || block != before);
+  const int start = 63 - __builtin_clzll(heads_of_runs & ((uint64_t(2) << lane) - 1));
+  const bool member = block >= 0 && start >= 1 && start <= 16 && lane <= 32;
+  const uint64_t members = __builtin_amdgcn_ballot_w64(member);
+  if (members == 0) return;
+
+  uint32_t* const scale_at = a.scales + ((int64_t)(member ? block : 0) * a.hkv + head) * 2 + side;
+  uint32_t old = 0;
+  if (member) old = *scale_at;
+
+  // ---- values
+  const uint16_t* src = (side ? a.v : a.k) + (int64_t)head * 128;
+  float x[kPasses][16];
+  uint32_t top[kPasses];
+#pragma unroll
+  for (int s = 0; s < kPasses; ++s) {
+    top[s] = 0;
+    if (((members >> (1 + 8 * s)) & 0xff) == 0) continue;
+    const int64_t r = min(r0 + 8 * s + g, (int64_t)a.rows - 1);
+    const uint16_t* at = src + r * a.kv_stride;
+    unpack16<BF16>(ldv(at + 8 * c), ldv(at + 64 + 8 * c), x[s]);
+  }
+#pragma unroll
+  for (int s = 0; s < kPasses; ++s) {
+    if (((members >> (1 + 8 * s)) & 0xff) == 0) continue;
+    if (FORM != Kv8Form::Store && side == 0) {
+      if constexpr (FORM == Kv8Form::NormRope) normalize16<BF16>(x[s], a.kw, c, a.eps);
+      const int at = __shfl(p, 1 + 8 * s + g, 64);
+      if (at >= 0) rotate16(x[s], a.table + (int64_t)at * 128 + 8 * c);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t bits = __float_as_uint(x[s][e]) & 0x7fffffffu;
+      top[s] = max(top[s], bits < kInfBits ? min(bits, __float_as_uint(kv8_cap<BF16>())) : 0u);
+    }
+    top[s] = max8(top[s]);
+  }
+
+  // ---- the runs' scales, from the rows' maxima
+  uint32_t amax = 0;
+#pragma unroll
+  for (int s = 0; s < kPasses; ++s) {
+    const uint32_t t = (uint32_t)__shfl((int)top[s], (8 * (lane - 1)) & 63, 64);
+    if (lane - 1 >= 8 * s && lane - 1 < 8 * s + 8) amax = t;
+  }
+  uint32_t written = member ? 1u << (slot & 15) : 0;
+  if (!member) amax = 0;
+#pragma unroll
+  for (int d = 1; d <= 16; d <<= 1) {  // over the lanes behind, within the run
+    const uint32_t am = (uint32_t)__shfl_down((int)amax, d, 64);
+    const uint32_t wr = (uint32_t)__shfl_down((int)written, d, 64);
+    const int st = __shfl_down(start, d, 64);
+    if (lane + d < 64 && st == start) {
+      amax = max(amax, am);
+      written |= wr;
+    }
+  }
+  amax = (uint32_t)__shfl((int)amax, start, 64);
+  written = (uint32_t)__shfl((int)written, start, 64);
+  old &= kInfBits;
+  if (old == kInfBits || (written & 1u)) old = 0;
+  const uint32_t scale = max(kv8_need(amax), old);
+  const bool leader = member && start == lane;
+  if (leader) *scale_at = scale;
+
+  // ---- the codes
+  uint8_t* cache = (side ? a.vc : a.kc) + (int64_t)head * 128;
+  const int64_t row_bytes = (int64_t)a.hkv * 128;
+#pragma unroll
+  for (int s = 0; s < kPasses; ++s) {
+    if (((members >> (1 + 8 * s)) & 0xff) == 0) continue;
+    const int from = 1 + 8 * s + g;
+    const float inv = kv8_inverse((uint32_t)__shfl((int)scale, from, 64));
+    const int to = __shfl(member ? slot : -1, from, 64);
+    const float cap = kv8_cap<BF16>();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float y = x[s][e];
+      // (what is not finite passes, and has no code but NaN's)
+      x[s][e] = (fabsf(y) > cap && fabsf(y) < __builtin_huge_valf() ? __builtin_copysignf(cap, y) : y) * inv;
+    }
+    if (to >= 0) {
+      uint8_t* dst = cache + (int64_t)to * row_bytes + 8 * c;
+      const u32x2 lo = {kv8_encode4(x[s][0], x[s][1], x[s][2], x[s][3]),
+                        kv8_encode4(x[s][4], x[s][5], x[s][6], x[s][7])};
+      const u32x2 hi = {kv8_encode4(x[s][8], x[s][9], x[s][10], x[s][11]),
+                        kv8_encode4(x[s][12], x[s][13], x[s][14], x[s][15])};
+      *reinterpret_cast<u32x2*>(dst) = lo;
+      *reinterpret_cast<u32x2*>(dst + 64) = hi;
+    }
+  }
+
+  // ---- earlier tokens of blocks whose scale grew: four lanes a token
+  uint64_t grown = __builtin_amdgcn_ballot_w64(leader && !(written & 1u) && scale > old);
+  while (grown != 0) {
+    const int l = __builtin_ctzll(grown);
+    grown &= grown - 1;
+    const int b = __builtin_amdgcn_readlane(block, l);
+    const uint32_t wr = (uint32_t)__builtin_amdgcn_readlane((int)written, l);
+    const int de = (__builtin_amdgcn_readlane((int)old, l) - __builtin_amdgcn_readlane((int)scale, l)) >> 23;
+    const float ratio = __builtin_ldexpf(1.f, de);
+    const int t = lane >> 2;
+    if (((wr >> t) & 1u) == 0) {
+      u32x4* codes = reinterpret_cast<u32x4*>(cache + ((int64_t)b * 16 + t) * row_bytes + 32 * (lane & 3));
+      u32x4 w[2] = {codes[0], codes[1]};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const auto f0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], false);
+          const auto f1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], true);
+          w[i][j] = kv8_encode4(f0[0] * ratio, f0[1] * ratio, f1[0] * ratio, f1[1] * ratio);
+        }
+      codes[0] = w[0];
+      codes[1] = w[1];
+    }
+  }
+}
+
+template <bool BF16, Kv8Form FORM>
+__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a) {
+  const int64_t wave = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  const int64_t n_kv = ((int64_t)a.rows + 15) / 16 * (2 * a.hkv);
+  if (wave < n_kv) {
+    kv8_window<BF16, FORM>(a, wave);
+  } else if constexpr (FORM != Kv8Form::Store) {
+    const int lane = threadIdx.x & 63;
+    kv8_query<BF16, FORM>(a, (wave - n_kv) * 8 + (lane >> 3), lane & 7);
+  }
+}
+
+template <Kv8Form FORM>
+static hipError_t kv8_launch(const Kv8Args& a, bool bf16, hipStream_t st) {
+  const int64_t n_kv = ((int64_t)a.rows + 15) / 16 * (2 * a.hkv);
+  const int64_t n_q = FORM == Kv8Form::Store ? 0 : ((int64_t)a.rows * a.hq + 7) / 8;
+  const int64_t grid = (n_kv + n_q + 3) / 4;
+  if (grid == 0) return hipSuccess;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (bf16) hipLaunchKernelGGL((kv8_append_kernel<true, FORM>), dim3((uint32_t)grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv8_append_kernel<false, FORM>), dim3((uint32_t)grid), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_store_kv8(const void* k, const void* v, void* kc, void* vc, float* scales, const int64_t* slots,
+                            int rows, int hkv, bool bf16, int cache_slots, hipStream_t st) {
+  Kv8Args a{};
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.kv_stride = (int64_t)hkv * 128;
+  a.kc = (uint8_t*)kc;
+  a.vc = (uint8_t*)vc;
+  a.scales = (uint32_t*)scales;
+  a.slots = slots;
+  a.rows = rows;
+  a.hkv = hkv;
+  a.cache_slots = cache_slots;
+  return kv8_launch<Kv8Form::Store>(a, bf16, st);
+}
+
+hipError_t launch_rope_append_kv8(void* q, const void* k, const void* v, void* kc, void* vc, float* scales,
+                                  const int64_t* pos, const int64_t* slots, const float* table, int rows, int hq,
+                                  int hkv, bool bf16, int max_pos, int cache_slots, hipStream_t st) {
+  Kv8Args a{};
+  a.q = (const uint16_t*)q;
+  a.q_out = (uint16_t*)q;
+  a.q_stride = (int64_t)hq * 128;
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.kv_stride = (int64_t)hkv * 128;
+  a.kc = (uint8_t*)kc;
+  a.vc = (uint8_t*)vc;
+  a.scales = (uint32_t*)scales;
+  a.pos = pos;
+  a.slots = slots;
+  a.table = table;
+  a.rows = rows;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.max_pos = max_pos;
+  a.cache_slots = cache_slots;
+  return kv8_launch<Kv8Form::Rope>(a, bf16, st);
+}
+
+hipError_t launch_norm_rope_append_kv8(const void* qkv, int64_t row_stride, const void* qw, const void* kw, float eps,
+                                       void* q_out, void* kc, void* vc, float* scales, const int64_t* pos,
+                                       const int64_t* slots, const float* table, int rows, int hq, int hkv, bool bf16,
+                                       int max_pos, int cache_slots, hipStream_t st) {
+  Kv8Args a{};
+  a.q = (const uint16_t*)qkv;
+  a.k = a.q + (int64_t)hq * 128;
+  a.v = a.k + (int64_t)hkv * 128;
+  a.q_stride = a.kv_stride = row_stride;
+  a.qw = (const uint16_t*)qw;
+  a.kw = (const uint16_t*)kw;
+  a.eps = eps;
+  a.q_out = (uint16_t*)q_out;
+  a.kc = (uint8_t*)kc;
+  a.vc = (uint8_t*)vc;
+  a.scales = (uint32_t*)scales;
+  a.pos = pos;
+  a.slots = slots;
+  a.table = table;
+  a.rows = rows;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.max_pos = max_pos;
+  a.cache_slots = cache_slots;
+  return kv8_launch<Kv8Form::NormRope>(a, bf16, st);
+}
+
+// Tokens of the cache as 16-bit rows: a thread takes 16 codes of K and of V
+// (16-byte loads, two 16-byte stores each).  Rows whose slot is outside the
+// cache are left as they are.
+template <bool BF16>
+__global__ __launch_bounds__(256) void kv8_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                       const float* __restrict__ scales,
+                                                       const int64_t* __restrict__ slots, uint16_t* __restrict__ k_out,
+                                                       uint16_t* __restrict__ v_out, int64_t total, int hkv,
+                                                       int cache_slots) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= total) return;
+  const int64_t unit = idx >> 3;  // (row, head)
+  const int c = (int)(idx & 7);
+  const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)unit / (uint32_t)hkv) : unit / hkv;
+  const int head = (int)(unit - row * hkv);
+  const int64_t slot = slots[row];
+  if (slot < 0 || slot >= cache_slots) return;
+  const int64_t from = (slot * hkv + head) * 128 + 16 * c;
+  const u32x4 kw = *reinterpret_cast<const u32x4*>(kc + from);
+  const u32x4 vw = *reinterpret_cast<const u32x4*>(vc + from);
+  const float* s = scales + ((slot >> 4) * hkv + head) * 2;
+  const float ks = s[0], vs = s[1];
+  const int64_t to = unit * 128 + 16 * c;
+  stv(k_out + to, kv8_decode8<BF16>(kw[0], kw[1], ks, ks));
+  stv(k_out + to + 8, kv8_decode8<BF16>(kw[2], kw[3], ks, ks));
+  stv(v_out + to, kv8_decode8<BF16>(vw[0], vw[1], vs, vs));
+  stv(v_out + to + 8, kv8_decode8<BF16>(vw[2], vw[3], vs, vs));
+}
+
+hipError_t launch_load_kv8(const void* kc, const void* vc, const float* scales, const int64_t* slots, void* k_out,
+                           void* v_out, int rows, int hkv, bool bf16, int cache_slots, hipStream_t st) {
+  const int64_t total = (int64_t)rows * hkv * 8;
+  if (total == 0) return hipSuccess;
+  const int64_t grid = (total + 255) / 256;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, scales,
+                       slots, (uint16_t*)k_out, (uint16_t*)v_out, total, hkv, cache_slots);
+  };
+  if (bf16) go(kv8_load_kernel<true>);
+  else go(kv8_load_kernel<false>);
+  return hipGetLastError();
+}
+
+}  // namespace feattn

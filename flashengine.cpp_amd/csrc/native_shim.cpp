@@ -92,4 +92,35 @@ void rope_store(void* q, const void* k, const void* v, void* kc, void* vc, const
                        cache_slots, stream));
 }
 
+void attention_kv8(AttentionPlan* plan, void* q, void* k, void* v, const float* scales, void* output, float* lse,
+                   bool causal, void* stream) {
+  if (plan == nullptr) throw std::runtime_error("feattn: null plan");
+  check(fe_attn_run_kv8(plan->plan, q, k, v, scales, output, lse, causal ? 1 : 0, stream));
+}
+
+void store_kv8(const void* k, const void* v, void* kc, void* vc, float* scales, const int64_t* slots, int rows,
+               int hkv, int dim, bool bf16, void* stream, int cache_slots) {
+  check(fe_store_kv8(k, v, kc, vc, scales, slots, rows, hkv, dim, bf16 ? 1 : 0, cache_slots, stream));
+}
+
+void rope_store_kv8(void* q, const void* k, const void* v, void* kc, void* vc, float* scales, const int64_t* pos,
+                    const int64_t* slots, const float* cache, int rows, int hq, int hkv, int dim, bool bf16,
+                    void* stream, int max_positions, int cache_slots) {
+  check(fe_rope_append_kv8(q, k, v, kc, vc, scales, pos, slots, cache, rows, hq, hkv, dim, bf16 ? 1 : 0,
+                           max_positions, cache_slots, stream));
+}
+
+void norm_rope_store_kv8(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, float eps,
+                         void* q_out, void* kc, void* vc, float* scales, const int64_t* pos, const int64_t* slots,
+                         const float* cache, int rows, int hq, int hkv, int dim, bool bf16, void* stream,
+                         int max_positions, int cache_slots) {
+  check(fe_norm_rope_append_kv8(qkv, row_stride, q_weight, k_weight, eps, q_out, kc, vc, scales, pos, slots, cache,
+                                rows, hq, hkv, dim, bf16 ? 1 : 0, max_positions, cache_slots, stream));
+}
+
+void load_kv8(const void* kc, const void* vc, const float* scales, const int64_t* slots, void* k_out, void* v_out,
+              int rows, int hkv, int dim, bool bf16, void* stream, int cache_slots) {
+  check(fe_load_kv8(kc, vc, scales, slots, k_out, v_out, rows, hkv, dim, bf16 ? 1 : 0, cache_slots, stream));
+}
+
 }  // namespace fe::cuda

@@ -42,6 +42,10 @@ C_SYMBOLS = (
     "fe_attn_version",
     "fe_attn_run_noalloc",
     "fe_attn_assign_shares",
+    "fe_attn_run_kv8",
+    "fe_store_kv8",
+    "fe_rope_append_kv8",
+    "fe_load_kv8",
 )
 
 # Every extern "C" symbol of include/fe_driver.h.
@@ -70,6 +74,7 @@ OPS_SYMBOLS = (
     "fe_silu_mul",
     "fe_accept",
     "fe_norm_rope_append",
+    "fe_norm_rope_append_kv8",
 )
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -115,6 +120,10 @@ def lib() -> ctypes.CDLL:
     L.fe_attn_plan_describe.argtypes = [_int] * 7 + [_i32p] * 4 + [_int, _int, _i32p]
     L.fe_attn_plan_dump.argtypes = [_int] * 7 + [_i32p] * 4 + [_int, _int, _int, _i32p, _int,
                                                              ctypes.POINTER(_int)]
+    L.fe_attn_run_kv8.argtypes = [_vp] * 7 + [_int, _vp]
+    L.fe_store_kv8.argtypes = [_vp] * 6 + [_int] * 5 + [_vp]
+    L.fe_rope_append_kv8.argtypes = [_vp] * 9 + [_int] * 7 + [_vp]
+    L.fe_load_kv8.argtypes = [_vp] * 6 + [_int] * 5 + [_vp]
     for name in C_SYMBOLS:
         getattr(L, name).restype = ctypes.c_char_p if name in (
             "fe_attn_last_error", "fe_attn_version") else _int
@@ -145,6 +154,7 @@ def lib() -> ctypes.CDLL:
     L.fe_silu_mul.argtypes = [_vp, _vp, _int, _int, _int, _vp]
     L.fe_accept.argtypes = [_vp, _vp, _vp, _int, _int, _vp]
     L.fe_norm_rope_append.argtypes = ([_vp, _i64, _vp, _vp, _f] + [_vp] * 6 + [_int] * 4 + [_int, _int, _int, _vp])
+    L.fe_norm_rope_append_kv8.argtypes = [_vp, _i64, _vp, _vp, _f] + [_vp] * 7 + [_int] * 7 + [_vp]
     for name in OPS_SYMBOLS:
         getattr(L, name).restype = _int
     _LIB = L
@@ -217,6 +227,12 @@ class Plan:
         _check(lib().fe_attn_run(self._h, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out),
                                  _ptr(lse), int(bool(causal)), _stream(stream)))
 
+    def run_kv8(self, q, k_cache, v_cache, scales, out, causal: bool = True, lse=None, stream=None) -> None:
+        """run on an 8-bit cache (fe_attn_run_kv8): e4m3 codes [blocks + 1][page][hkv][128]
+        and fp32 scales [(blocks + 1) * page / 16][hkv][2]."""
+        _check(lib().fe_attn_run_kv8(self._h, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(scales), _ptr(out),
+                                     _ptr(lse), int(bool(causal)), _stream(stream)))
+
     def lists(self, causal: bool = True) -> PlanLists:
         """What the latest prepare planned for run(causal=causal) (fe_attn_plan_lists)."""
         out = (ctypes.c_int32 * 8)()
@@ -266,6 +282,28 @@ def rope_append(q, k, v, k_cache, v_cache, pos, slots, cache, rows: int, hq: int
     _check(lib().fe_rope_append(_ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(pos),
                                 _ptr(slots), _ptr(cache), rows, hq, hkv, dim, int(bool(bf16)),
                                 max_positions, cache_slots, _stream(stream)))
+
+
+def store_kv8(k, v, k_cache, v_cache, scales, slots, rows: int, hkv: int, dim: int, bf16: bool, cache_slots: int,
+              stream=None) -> None:
+    """Store of k, v [rows][hkv][128] into an 8-bit cache (fe_store_kv8)."""
+    _check(lib().fe_store_kv8(_ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(scales), _ptr(slots), rows, hkv,
+                              dim, int(bool(bf16)), cache_slots, _stream(stream)))
+
+
+def rope_append_kv8(q, k, v, k_cache, v_cache, scales, pos, slots, cache, rows: int, hq: int, hkv: int, dim: int,
+                    bf16: bool, max_positions: int, cache_slots: int, stream=None) -> None:
+    """Fused rope + store into an 8-bit cache (q rotated in place)."""
+    _check(lib().fe_rope_append_kv8(_ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(scales), _ptr(pos),
+                                    _ptr(slots), _ptr(cache), rows, hq, hkv, dim, int(bool(bf16)), max_positions,
+                                    cache_slots, _stream(stream)))
+
+
+def load_kv8(k_cache, v_cache, scales, slots, k_out, v_out, rows: int, hkv: int, dim: int, bf16: bool,
+             cache_slots: int, stream=None) -> None:
+    """Tokens of an 8-bit cache as 16-bit rows [rows][hkv][128] (fe_load_kv8)."""
+    _check(lib().fe_load_kv8(_ptr(k_cache), _ptr(v_cache), _ptr(scales), _ptr(slots), _ptr(k_out), _ptr(v_out), rows,
+                             hkv, dim, int(bool(bf16)), cache_slots, _stream(stream)))
 
 
 def describe(hq, hkv, dim, page, max_batch, max_pages, blocks, qo, kv, pages, last, batch, rows):
@@ -472,3 +510,13 @@ def norm_rope_append(qkv, row_stride: int, q_weight, k_weight, eps: float, q_out
                                      _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(pos), _ptr(slots), _ptr(cache),
                                      rows, hq, hkv, dim, int(bool(bf16)), max_positions, cache_slots,
                                      _stream(stream)))
+
+
+def norm_rope_append_kv8(qkv, row_stride: int, q_weight, k_weight, eps: float, q_out, k_cache, v_cache, scales, pos,
+                         slots, cache, rows: int, hq: int, hkv: int, bf16: bool, max_positions: int,
+                         cache_slots: int, dim: int = 128, stream=None) -> None:
+    """q/k RMSNorm + RoPE + append to an 8-bit cache in one pass (fe_norm_rope_append_kv8)."""
+    _check(lib().fe_norm_rope_append_kv8(_ptr(qkv), row_stride, _ptr(q_weight), _ptr(k_weight), float(eps),
+                                         _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(scales), _ptr(pos),
+                                         _ptr(slots), _ptr(cache), rows, hq, hkv, dim, int(bool(bf16)),
+                                         max_positions, cache_slots, _stream(stream)))

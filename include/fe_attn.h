@@ -154,6 +154,68 @@ int fe_attn_run_noalloc(const void* q, const void* k_cache, const void* v_cache,
                         int hkv, int dim, int page, int blocks, int bf16,
                         void* stream);
 
+/* --- 8-bit caches ---------------------------------------------------------
+ * No counterpart in the reference.  A cache of half the bytes:
+ *   k/v cache    [blocks+1][page][hkv][128]            e4m3 codes (OCP; 0x7f
+ *                and 0xff are NaN, there is no infinity), one byte each
+ *   scales       fp32 [(blocks+1)*page/16][hkv][2]     a power of two for K
+ *                and one for V of every 16 consecutive slots (a scale block)
+ *                and head, 8-byte aligned; slot s belongs to block s / 16
+ * A cached value is code * scale.  The append functions below write codes and
+ * scales; a cache filled by other means must hold finite powers of two (the
+ * kernels take a scale's exponent only) with values inside the 16-bit type's
+ * range.  Neither array needs to be initialised: what no call has written is
+ * never used.
+ *
+ * Appending.  For every scale block and head that a call writes, K and V each:
+ *   need  = the smallest power of two s >= 2^-118 with |x| <= 448 s for every
+ *           finite value x that the call puts there
+ *   scale = need if the call writes the block's first slot, which starts the
+ *           block (what its other slots held is lost); else max(scale, need),
+ *           and where that grows, the codes already there are rescaled
+ *   code  = x / scale rounded to nearest even from fp32, once.  Infinities
+ *           and NaNs become NaN; magnitudes above 61440 (fp16) or 1.875 * 2^127
+ *           (bf16), which would round up to infinity, become that.
+ * So that a block's slots are filled in order, as a sequence's positions do.
+ * The rows of a call that go to one block must follow one another in the call,
+ * with no other row (nor a skipped one) between them, in any order, as the rows
+ * of a sequence do, and their slots must be distinct: otherwise the contents of
+ * the blocks concerned are unspecified.  Rows with slot < 0 or >= cache_slots are
+ * skipped, those with a position outside [0, max_positions) are not rotated.
+ * cache_slots must be a multiple of 16, dim 128; tensors (the rope table too)
+ * 16-byte aligned, else FE_EINVAL.  May be captured into a HIP graph. */
+
+/* fe_attn_run on an 8-bit cache: the same plan, prepared the same way (one
+ * prepare serves both kinds of cache), the same masks, rows and outputs.  Scores
+ * and sums are exact products of 16-bit q and the cached values, accumulated in
+ * fp32.  Slots outside the visible ranges are not used, whatever codes or
+ * scales they hold. */
+int fe_attn_run_kv8(fe_attn_plan* plan, const void* q, const void* k_cache,
+                    const void* v_cache, const float* scales, void* out,
+                    float* lse, int causal, void* stream);
+
+/* fe_store into an 8-bit cache: k, v [rows][hkv][128] 16-bit. */
+int fe_store_kv8(const void* k, const void* v, void* k_cache, void* v_cache,
+                 float* scales, const int64_t* slots, int rows, int hkv,
+                 int dim, int bf16, int cache_slots, void* stream);
+
+/* fe_rope_append into an 8-bit cache.  q is rotated in place, bit-identical to
+ * fe_rope; k and v are read only, and k is rotated in fp32 and rounded once, to
+ * its codes. */
+int fe_rope_append_kv8(void* q, const void* k, const void* v, void* k_cache,
+                       void* v_cache, float* scales, const int64_t* pos,
+                       const int64_t* slots, const float* cache, int rows,
+                       int hq, int hkv, int dim, int bf16, int max_positions,
+                       int cache_slots, void* stream);
+
+/* Cached tokens as 16-bit rows (a prefix handed to another cache, say): k_out
+ * and v_out [rows][hkv][128] receive the values at slots[r], rounded to
+ * nearest even (exact but below the type's smallest normal value).  Rows with
+ * slot < 0 or >= cache_slots are left as they are. */
+int fe_load_kv8(const void* k_cache, const void* v_cache, const float* scales,
+                const int64_t* slots, void* k_out, void* v_out, int rows,
+                int hkv, int dim, int bf16, int cache_slots, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* fe_attn_last_error(void);
 

@@ -36,4 +36,19 @@ void accept(const int64_t* draft, const int64_t* verify, int64_t* committed, int
 void norm_rope_store(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, float eps,
                      void* q_out, void* kc, void* vc, const int64_t* pos, const int64_t* slots, const float* cache,
                      int rows, int hq, int hkv, int dim, bool bf16, void* stream, int max_positions, int cache_slots);
+// The same on an 8-bit cache of e4m3 codes with a power of two for every 16
+// slots and head (fe_attn.h: 8-bit caches).
+void attention_kv8(AttentionPlan* plan, void* q, void* k, void* v, const float* scales, void* output, float* lse,
+                   bool causal, void* stream);
+void store_kv8(const void* k, const void* v, void* kc, void* vc, float* scales, const int64_t* slots, int rows,
+               int hkv, int dim, bool bf16, void* stream, int cache_slots);
+void rope_store_kv8(void* q, const void* k, const void* v, void* kc, void* vc, float* scales, const int64_t* pos,
+                    const int64_t* slots, const float* cache, int rows, int hq, int hkv, int dim, bool bf16,
+                    void* stream, int max_positions, int cache_slots);
+void norm_rope_store_kv8(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, float eps,
+                         void* q_out, void* kc, void* vc, float* scales, const int64_t* pos, const int64_t* slots,
+                         const float* cache, int rows, int hq, int hkv, int dim, bool bf16, void* stream,
+                         int max_positions, int cache_slots);
+void load_kv8(const void* kc, const void* vc, const float* scales, const int64_t* slots, void* k_out, void* v_out,
+              int rows, int hkv, int dim, bool bf16, void* stream, int cache_slots);
 }  // namespace fe::cuda

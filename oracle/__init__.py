@@ -18,6 +18,8 @@ Modules:
   norm_ops        numpy restatement of RMSNorm, the SiLU-gated product,
                   greedy acceptance and the fused q/k norm + rope + append
                   (src/cuda_kernels.cu:11-18,25, src/cuda_model.cpp:91-95).
+  kv8             the 8-bit paged KV cache (codes, scales, append, load,
+                  attention) in 64 bits.
 
 Pinning (what each function is checked against) is listed in each module's
 docstring and exercised by tests/test_oracle_*.py.
