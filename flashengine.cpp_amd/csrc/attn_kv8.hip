@@ -684,17 +684,42 @@ constexpr int kTile8Stage = 8 * kTile8Block;
 constexpr int kTile8Raw = 2 * kTile8Stage;           // offset of the wavefronts' code regions
 constexpr int kTile8Lds = kTile8Raw + 4 * 4096;      // 80 KB: two workgroups a compute unit
 
+// The lane's index, from the hardware: neither it nor what follows from it is
+// held in registers through items of the other kind.
+__device__ __forceinline__ int fresh_lane() {
+  uint32_t zero;
+  asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
+
 struct Tile8Lanes {
   uint32_t goff[2];
   uint32_t k_lds[4], v_lds[8];
 };
+
+__device__ __forceinline__ Tile8Lanes tile8_lanes(const AttnArgs& a, int lane) {
+  const int J = lane >> 4, L = lane & 15;
+  const int row_bytes = a.hkv * kHeadDim;
+  Tile8Lanes tl;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)((8 * r + (lane >> 3)) * row_bytes + 16 * (lane & 7));
+#pragma unroll
+  for (int s = 0; s < 4; ++s) tl.k_lds[s] = (uint32_t)(16 * (16 * L + (((4 * s + J) ^ L) & 15)));
+  const int k = L >> 2, m = L & 3, t = 4 * J + k;
+#pragma unroll
+  for (int db = 0; db < 8; ++db) {
+    const int c = 2 * db + (m >> 1);
+    tl.v_lds[db] = (uint32_t)(16 * (16 * t + ((c ^ (2 * t)) & 15)) + 8 * (m & 1));
+  }
+  return tl;
+}
 
 // Requests the codes of this wavefront's block (tokens T + 16 wave ..) of item
 // w's tile at T, and returns its scales; blocks at or past the item end are
 // skipped.
 template <bool STREAM>
 __device__ __forceinline__ f32x2 tile8_copy(const AttnArgs& a, const WorkItem& w, const SeqInfo& s,
-                                             const Tile8Lanes& tl, uint32_t lbase, int wave, int T) {
+                                             const uint32_t (&goff)[2], uint32_t lbase, int wave, int T) {
   const int tok = T + 16 * wave;
   if (tok >= w.t1) return f32x2{1.f, 1.f};
   const int pshift = a.page_shift;
@@ -706,9 +731,9 @@ __device__ __forceinline__ f32x2 tile8_copy(const AttnArgs& a, const WorkItem& w
   const char* vb = reinterpret_cast<const char*>(a.vc) + off;
   const uint32_t raw = lbase + (uint32_t)(kTile8Raw + wave * 4096);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) lds_dma16<STREAM>(kb, tl.goff[r], raw + 1024 * r);
+  for (int r = 0; r < 2; ++r) lds_dma16<STREAM>(kb, goff[r], raw + 1024 * r);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) lds_dma16<STREAM>(vb, tl.goff[r], raw + 2048 + 1024 * r);
+  for (int r = 0; r < 2; ++r) lds_dma16<STREAM>(vb, goff[r], raw + 2048 + 1024 * r);
   return ldc_scales(a.scales, blk * (size_t)a.hkv + (size_t)w.kvh);
 }
 
@@ -867,8 +892,8 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
       }
     }
     __syncthreads();  // the tile is in LDS, its codes are read, the other tile is free
-    if (T + kTileTokens < t1) scales = tile8_copy<STREAM>(a, w, s, tl, lbase, wave, T + kTileTokens);
-    else if (has_next) scales = tile8_copy<STREAM>(a, wn, sn, tl, lbase, wave, wn.t0);
+    if (T + kTileTokens < t1) scales = tile8_copy<STREAM>(a, w, s, tl.goff, lbase, wave, T + kTileTokens);
+    else if (has_next) scales = tile8_copy<STREAM>(a, wn, sn, tl.goff, lbase, wave, wn.t0);
     if (wave_on) {
       if (T + kTileTokens - 1 <= lim_min) compute(st, T, std::false_type{});
       else compute(st, T, std::true_type{});
@@ -903,39 +928,360 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
   return stage;
 }
 
+// ---------------------------------------------------------------------------
+// Items of at most 64 columns (draft blocks, verify rows): HBM bound
+// ---------------------------------------------------------------------------
+// Here each wavefront owns tokens instead of columns: steps of 32 tokens go to
+// the four wavefronts in turn, every wavefront computes all 64 columns on its
+// own, from codes that it alone copies, converts and reads once, with no
+// barrier from the first step to the last; the four results are combined in
+// LDS at the end of the item.  Q (64 columns, 16 KB) lies in LDS.
+constexpr int kBlk8Q = 64 * 256;
+constexpr int kBlk8Units = 3;
+constexpr int kBlk8Wave = kBlk8Units * kKv8Slot;
+constexpr int kBlk8Stats = 4 * 16384;  // combining: 32 columns x 128 fp32 of each wavefront, then the statistics
+static_assert(kBlk8Stats + 4 * 64 * 8 <= kTile8Lds && kBlk8Q + 4 * kBlk8Wave <= kTile8Lds, "");
+
 template <bool BF16, bool CAUSAL, bool STREAM>
+__device__ __forceinline__ void block8_item(const AttnArgs& a, const WorkItem& w, const SeqInfo& s, uint32_t lbase,
+                                            int wave, int lane) {
+  constexpr int NCB = 4;
+  const int J = lane >> 4;
+  const int L = lane & 15;
+  const int G = a.group;
+  const int kvh = w.kvh;
+  const int t0 = w.t0;
+  const int t1 = w.t1;
+  const int ncols = w.nq * G;
+  const int pshift = a.page_shift;
+  const int pmask = (1 << pshift) - 1;
+  const int row_bytes = a.hkv * kHeadDim;
+  const uint32_t ring = lbase + (uint32_t)(kBlk8Q + wave * kBlk8Wave);
+  typedef __attribute__((address_space(3))) float lds_f32;
+  typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+
+  uint32_t k_goff[2], v_goff[4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int t = 8 * r + (lane >> 3);
+    k_goff[r] = (uint32_t)(t * row_bytes + 16 * ((lane & 7) ^ swz_k(t)));
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int t = 8 * r + (lane >> 3);
+    v_goff[r] = (uint32_t)((t & 15) * row_bytes + 16 * ((lane & 7) ^ swz_v(t)));
+  }
+  // Operand reads: chunk J of row L (K; J + 4: ^ 64), chunk 2 J of row L (Q; the
+  // k-step 2 i + h: ^ 16 (8 i + h)), v_operand_addr's of dim block 0 (db: ^ 16 db).
+  uint32_t k_at = (uint32_t)(128 * L + 16 * (J ^ swz_k(L)));
+  uint32_t q_at = (uint32_t)(256 * L + 16 * ((2 * J) ^ L));
+  uint32_t v_at;
+  {
+    const int k = L >> 1, t = k < 4 ? 4 * J + k : 16 + 4 * J + k - 4;
+    v_at = (uint32_t)(128 * t + 16 * swz_v(t) + 8 * (L & 1));
+  }
+
+  // Q: wavefront w copies column block w; columns past the item repeat its first.
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int n = 4 * r + J;
+    const int col = 16 * wave + n;
+    const int nn = col < ncols ? col : 0;
+    lds_dma16(a.q + ((size_t)(w.q0 + nn / G) * a.hq + kvh * G + nn % G) * kHeadDim + 8 * (L ^ n),
+              lbase + (uint32_t)(4096 * wave + 1024 * r));
+  }
+
+  // ---- copy side: K, then V of this wavefront's steps (tokens c_tok .. + 31)
+  auto page_id = [&](int tok) { return ldc(a.pages, s.page_off + (tok >> pshift)); };
+  auto block_of = [&](int tok, int pg) { return ((size_t)pg << (pshift - 4)) + (size_t)((tok & pmask) >> 4); };
+  int c_tok = t0 + 32 * wave;
+  bool c_live = c_tok < t1, c_key = true;
+  int pg0 = 0, pg1 = 0;
+  if (c_live) {
+    pg0 = page_id(c_tok);
+    pg1 = page_id(min(c_tok + 16, t1 - 1));
+  }
+  size_t blk0 = 0, blk1 = 0;
+  int issued = 0, consumed = 0, c_slot = 0, r_slot = 0;
+  auto issue_codes = [&](const void* cache, const uint32_t (&goff)[4], int side, uint32_t dst) {
+    const char* base = reinterpret_cast<const char*>(cache) + (size_t)kvh * kHeadDim;
+    const char* b0 = base + blk0 * (size_t)(16 * row_bytes);
+    const char* b1 = base + blk1 * (size_t)(16 * row_bytes);
+    lds_dma16<STREAM>(b0, goff[0], dst);
+    lds_dma16<STREAM>(b0, goff[1], dst + 1024);
+    lds_dma16<STREAM>(b1, goff[2], dst + 2048);
+    lds_dma16<STREAM>(b1, goff[3], dst + 3072);
+    const size_t at = (lane & 1) ? blk1 : blk0;
+    lds_dma4(a.scales + 2 * (at * (size_t)a.hkv + (size_t)kvh) + side, dst + kKv8Unit);
+  };
+  auto refill = [&]() {  // (the caller has waited for its reads of the slot freed last)
+    while (c_live && issued - consumed < kBlk8Units) {
+      const uint32_t dst = ring + (uint32_t)(c_slot * kKv8Slot);
+      if (c_key) {
+        blk0 = block_of(c_tok, pg0);
+        blk1 = c_tok + 16 < t1 ? block_of(c_tok + 16, pg1) : blk0;
+        const uint32_t kg[4] = {k_goff[0], k_goff[1], k_goff[0], k_goff[1]};
+        issue_codes(a.kc, kg, 0, dst);
+        if (c_tok + 128 < t1) {
+          pg0 = page_id(c_tok + 128);
+          pg1 = page_id(min(c_tok + 144, t1 - 1));
+        }
+      } else {
+        issue_codes(a.vc, v_goff, 1, dst);
+        c_tok += 128;
+        c_live = c_tok < t1;
+      }
+      c_key = !c_key;
+      ++issued;
+      c_slot = c_slot + 1 == kBlk8Units ? 0 : c_slot + 1;
+    }
+  };
+  refill();
+
+  int lim[NCB];
+  int lim_min = 1 << 30;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int n = 16 * cb + L;
+    lim[cb] = -1;
+    if (n < ncols) {
+      lim[cb] = min(CAUSAL ? s.len - s.qlen + (w.q0 + n / G - s.qo) : s.len - 1, t1 - 1);
+      lim_min = min(lim_min, lim[cb]);
+    }
+  }
+#pragma unroll
+  for (int o_ = 8; o_ >= 1; o_ >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o_, 64));
+  lim_min = uniform(lim_min);
+
+  float m[NCB], lsum[NCB];
+  f32x4 o[8][NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    m[cb] = kNegInf;
+    lsum[cb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  wait_units<kBlk8Units, 5>(issued);  // Q
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+
+  for (int tok = t0 + 32 * wave; tok < t1; tok += 128) {
+    asm volatile("" : "+v"(k_at), "+v"(q_at), "+v"(v_at));  // (the derived addresses are not to be held)
+    // ---- S^T
+    wait_units<kBlk8Units, 5>(issued - consumed - 1);
+    const uint32_t kst = ring + (uint32_t)(r_slot * kKv8Slot);
+    r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
+    const f32x2 ks = *(lds_f32x2*)(uintptr_t)(kst + kKv8Unit);
+    u32x4 kw[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) kw[i][tb] = lds_read16(kst + 2048 * tb + (k_at ^ (64 * i)));
+    u32x4 qf[2][NCB];  // this k-step's and the next one's
+    auto read_q = [&](int k) {
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb)
+        qf[k & 1][cb] = lds_read16(lbase + (q_at ^ (16 * (8 * (k >> 1) + (k & 1)))) + 4096 * cb);
+    };
+    read_q(0);
+    f32x4 sc[2][NCB];
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k < 3) read_q(k + 1);
+      __builtin_amdgcn_sched_barrier(0);  // (else the reads sink to their use, behind a full LDS latency each)
+      u32x4 kf[2];
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+        kf[tb] = kv8_decode8<BF16>(kw[k >> 1][tb][2 * (k & 1)], kw[k >> 1][tb][2 * (k & 1) + 1], ks[tb], ks[tb]);
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) sc[tb][cb] = mfma16<BF16>(kf[tb], qf[k & 1][cb], sc[tb][cb]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_lds();
+    consumed += 1;
+    refill();
+
+    // ---- softmax
+    if (tok + 31 > lim_min) {
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
+    }
+    // The statistics first: V^T operands are read ahead of the exponentials.
+    float alpha[NCB];
+    bool any_up = false;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[tb][cb][r]);
+      mx = max_x32(max_x16(mx));
+      const float mt = mx * a.scale_log2;
+      const bool up = mt > m[cb] + 8.f;  // lazy reference maximum, p <= 2^8
+      alpha[cb] = up ? fast_exp2(m[cb] - mt) : 1.f;
+      if (up) m[cb] = mt;
+      any_up = any_up || up;
+    }
+    if (__builtin_amdgcn_ballot_w64(any_up) != 0) {
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        lsum[cb] *= alpha[cb];
+#pragma unroll
+        for (int db = 0; db < 8; ++db) o[db][cb] *= alpha[cb];
+      }
+    }
+    wait_units<kBlk8Units, 5>(issued - consumed - 1);
+    const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
+    r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
+    if (t1 - tok < 32) {
+      // rows past the item end: zero (0 * stale must stay 0)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int q = lane + 64 * u;
+        if ((q >> 3) >= t1 - tok) lds_zero16(vst + 16 * q);
+      }
+    }
+    const f32x2 vs = *(lds_f32x2*)(uintptr_t)(vst + kKv8Unit);
+    u32x2 vw[8];
+#pragma unroll
+    for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + (v_at ^ (16 * db)));
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 pf[NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+      float x[2][4];
+      float ps = 0.f;
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m_use));
+          ps += x[tb][r];
+        }
+      lsum[cb] += ps;
+      pf[cb] = u32x4{pack2<BF16>(x[0][0], x[0][1]), pack2<BF16>(x[0][2], x[0][3]), pack2<BF16>(x[1][0], x[1][1]),
+                     pack2<BF16>(x[1][2], x[1][3])};
+    }
+
+    // ---- O^T
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      const u32x4 vf = kv8_decode8<BF16>(vw[db][0], vw[db][1], vs[0], vs[1]);
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[cb], o[db][cb]);
+    }
+    wait_lds();
+    consumed += 1;
+    refill();
+  }
+
+  // ---- combine, 32 columns a round: row = column, 16-byte chunk c (dims 4 c
+  // ..) at chunk position c ^ (column % 16)
+  const uint32_t mine = lbase + (uint32_t)(16384 * wave);
+  const uint32_t stats = lbase + kBlk8Stats;
+  const int c = lane & 31;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) lsum[cb] = sum_x32(sum_x16(lsum[cb]));
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (32 * half < ncols) {
+      __syncthreads();  // the steps' (the other half's) reads are done
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int cb = 2 * half + i;
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+          *(lds_f32x4*)(uintptr_t)(mine + (uint32_t)(512 * (16 * i + L) + 16 * ((4 * db + J) ^ L))) = o[db][cb];
+        if (J == 0) {
+          const f32x2 st = {m[cb], lsum[cb]};
+          *(lds_f32x2*)(uintptr_t)(stats + (uint32_t)(8 * (64 * wave + 16 * cb + L))) = st;
+        }
+      }
+      __syncthreads();
+      for (int n = 2 * wave + (lane >> 5); n < 32; n += 8) {
+        const int col = 32 * half + n;
+        if (col >= ncols) break;
+        f32x2 st[4];
+        float top = kNegInf;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          st[v] = *(lds_f32x2*)(uintptr_t)(stats + (uint32_t)(8 * (64 * v + col)));
+          top = fmaxf(top, st[v][0]);
+        }
+        const float base = top == kNegInf ? 0.f : top;
+        float ls = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float wt = fast_exp2(st[v][0] - base);
+          ls += st[v][1] * wt;
+          acc += *(lds_f32x4*)(uintptr_t)(lbase + (uint32_t)(16384 * v + 512 * n + 16 * (c ^ (n & 15)))) * wt;
+        }
+        const float inv = ls > 0.f ? 1.f / ls : 0.f;
+        const float l2 = ls > 0.f ? top + __log2f(ls) : kNegInf;
+        const int r = col / G, head = kvh * G + (col - r * G);
+        const bool whole = w.part < 0;
+        const size_t oi = (size_t)(whole ? w.q0 + r : w.part + r) * a.hq + head;
+        const u32x2 v2 = {pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
+        *reinterpret_cast<u32x2*>((whole ? a.out : a.part_o) + oi * kHeadDim + 4 * c) = v2;
+        if (c == 0) {
+          if (!whole) a.part_lse[oi] = l2;
+          else if (a.lse != nullptr) a.lse[oi] = l2 * kLn2;
+        }
+      }
+    }
+  }
+}
+
+// Narrow: every item has at most 64 columns.  Wide: any items, as tiles.  Any:
+// the launch of a graph plan, whose later prepares may bring either kind.
+// (One kernel with all paths for the eager launches too takes 262 us for 8192
+// prompt tokens, 234 without the narrow items' path beside it.)
+enum class Tile8 { Narrow, Wide, Any };
+
+template <bool BF16, bool CAUSAL, bool STREAM, Tile8 KIND>
 __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t dsm[];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = uniform(tid >> 6);
-  const int J = lane >> 4;
-  const int L = lane & 15;
   const int n_items = uniform(*a.n_items);
-  const int row_bytes = a.hkv * kHeadDim;
   const uint32_t lbase = (uint32_t)(uintptr_t)dsm;
 
   Tile8Lanes tl;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)((8 * r + (lane >> 3)) * row_bytes + 16 * (lane & 7));
-#pragma unroll
-  for (int s = 0; s < 4; ++s) tl.k_lds[s] = (uint32_t)(16 * (16 * L + (((4 * s + J) ^ L) & 15)));
-  {
-    const int k = L >> 2, m = L & 3, t = 4 * J + k;
-#pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      const int c = 2 * db + (m >> 1);
-      tl.v_lds[db] = (uint32_t)(16 * (16 * t + ((c ^ (2 * t)) & 15)) + 8 * (m & 1));
-    }
-  }
+  if constexpr (KIND == Tile8::Wide) tl = tile8_lanes(a, lane);
 
-  int it = ldc(a.tile_off, blockIdx.x);
-  const int end = min(ldc(a.tile_off, blockIdx.x + 1), n_items);
+  // Narrow: workgroups of one XCD (every eighth) take neighbouring shares, the
+  // kv heads of one token range where the list is an equal cut, so that an
+  // XCD's L2 channels see all of a page's lines instead of one head's (32
+  // draft blocks over 2048..16384 tokens: 147 us a call, 156 in plain order).
+  const int n_wg = (int)gridDim.x;
+  const int b = KIND == Tile8::Narrow && n_wg % 8 == 0 ? (int)(blockIdx.x % 8) * (n_wg / 8) + (int)blockIdx.x / 8
+                                                        : (int)blockIdx.x;
+  int it = ldc(a.tile_off, b);
+  const int end = min(ldc(a.tile_off, b + 1), n_items);
   if (it >= end) return;
   WorkItem w = ldc_item(a.items, it);
   SeqInfo s = ldc_seq(a.seqs, w.seq);
-  f32x2 scales = tile8_copy<STREAM>(a, w, s, tl, lbase, wave, w.t0);
+  f32x2 scales = {1.f, 1.f};
   int stage = 0;
+  bool primed = false;  // w's first tile was requested during the item before
   for (;;) {
     const int nit = it + 1;
     const bool has_next = nit < end;
@@ -945,11 +1291,24 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
       wn = ldc_item(a.items, nit);
       sn = ldc_seq(a.seqs, wn.seq);
     }
-    if (w.nq * a.group <= 64)
-      stage = tile8_item<BF16, CAUSAL, 1, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
-    else
-      stage = tile8_item<BF16, CAUSAL, 2, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
+    if constexpr (KIND == Tile8::Wide) {
+      if (!primed) scales = tile8_copy<STREAM>(a, w, s, tl.goff, lbase, wave, w.t0);
+      primed = has_next;
+      if (w.nq * a.group <= 64)
+        stage = tile8_item<BF16, CAUSAL, 1, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
+      else
+        stage = tile8_item<BF16, CAUSAL, 2, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
+    } else if (KIND == Tile8::Narrow || w.nq * a.group <= 64) {
+      block8_item<BF16, CAUSAL, STREAM>(a, w, s, lbase, wave, fresh_lane());
+    } else if constexpr (KIND == Tile8::Any) {
+      const int ln = fresh_lane();
+      const Tile8Lanes tw = tile8_lanes(a, ln);
+      if (!primed) scales = tile8_copy<STREAM>(a, w, s, tw.goff, lbase, wave, w.t0);
+      primed = has_next && wn.nq * a.group > 64;
+      stage = tile8_item<BF16, CAUSAL, 2, STREAM>(a, w, s, primed, wn, sn, tw, lbase, wave, ln, stage, scales);
+    }
     if (!has_next) break;
+    if (!primed) __syncthreads();  // the next item lays out LDS anew
     it = nit;
     w = wn;
     s = sn;
@@ -1015,24 +1374,34 @@ hipError_t launch_decode_kv8(const AttnArgs& a, bool bf16, int waves, int ncb, i
               : decode8_waves<false>(a, waves, ncb, causal, any, grid, st);
 }
 
-template <bool BF16, bool CAUSAL, bool STREAM>
+template <bool BF16, bool CAUSAL, bool STREAM, Tile8 KIND>
 static hipError_t tile8_launch(const AttnArgs& a, int grid, hipStream_t st) {
   static std::atomic<uint64_t> lds_ok{0};
-  const hipError_t e = allow_lds((const void*)attn_tile_kv8_kernel<BF16, CAUSAL, STREAM>, kTile8Lds, lds_ok);
+  const hipError_t e = allow_lds((const void*)attn_tile_kv8_kernel<BF16, CAUSAL, STREAM, KIND>, kTile8Lds, lds_ok);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((attn_tile_kv8_kernel<BF16, CAUSAL, STREAM>), dim3(grid), dim3(256), kTile8Lds, st, a);
+  hipLaunchKernelGGL((attn_tile_kv8_kernel<BF16, CAUSAL, STREAM, KIND>), dim3(grid), dim3(256), kTile8Lds, st, a);
   return hipGetLastError();
 }
 
-hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, int grid, hipStream_t st) {
-  auto go = [&](auto bf, auto ca) {
-    constexpr bool B = decltype(bf)::value, C = decltype(ca)::value;
-    return stream ? tile8_launch<B, C, true>(a, grid, st) : tile8_launch<B, C, false>(a, grid, st);
+template <bool BF16, bool CAUSAL>
+static hipError_t tile8_kind(const AttnArgs& a, bool stream, bool any, bool narrow, int grid, hipStream_t st) {
+  auto go = [&](auto streamed) {
+    constexpr bool S = decltype(streamed)::value;
+    if (any) return tile8_launch<BF16, CAUSAL, S, Tile8::Any>(a, grid, st);
+    return narrow ? tile8_launch<BF16, CAUSAL, S, Tile8::Narrow>(a, grid, st)
+                  : tile8_launch<BF16, CAUSAL, S, Tile8::Wide>(a, grid, st);
   };
-  using T = std::true_type;
-  using F = std::false_type;
-  if (bf16) return causal ? go(T{}, T{}) : go(T{}, F{});
-  return causal ? go(F{}, T{}) : go(F{}, F{});
+  return stream ? go(std::true_type{}) : go(std::false_type{});
+}
+
+// any: a graph plan's launch; else narrow: every item has at most 64 columns.
+hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, bool any, bool narrow, int grid,
+                           hipStream_t st) {
+  if (bf16)
+    return causal ? tile8_kind<true, true>(a, stream, any, narrow, grid, st)
+                  : tile8_kind<true, false>(a, stream, any, narrow, grid, st);
+  return causal ? tile8_kind<false, true>(a, stream, any, narrow, grid, st)
+                : tile8_kind<false, false>(a, stream, any, narrow, grid, st);
 }
 
 }  // namespace feattn

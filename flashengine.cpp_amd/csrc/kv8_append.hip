@@ -67,58 +67,96 @@ __device__ __forceinline__ void unpack16(u32x4 lo, u32x4 hi, float (&x)[16]) {
   }
 }
 
-template <bool BF16>
-__device__ __forceinline__ void normalize16(float (&x)[16], const uint16_t* w, int c, float eps) {
-  float s = 0.f;
+// Normalization and rotation stay in fp32 up to the one rounding at the end;
+// sums in pairs and fused products keep them within a few 2^-24.
+__device__ __forceinline__ float rms16(const float (&x)[16], float eps) {
+  float s[4];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) s = __builtin_fmaf(x[e], x[e], s);
-  const float r = rsqrtf(sum8(s) * (1.f / 128.f) + eps);
-  float g[16];
-  unpack16<BF16>(ldv(w + 8 * c), ldv(w + 64 + 8 * c), g);
+  for (int i = 0; i < 4; ++i) {
+    s[i] = x[4 * i] * x[4 * i];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] = x[e] * r * g[e];
+    for (int e = 1; e < 4; ++e) s[i] = __builtin_fmaf(x[4 * i + e], x[4 * i + e], s[i]);
+  }
+  return rsqrtf(sum8((s[0] + s[1]) + (s[2] + s[3])) * (1.f / 128.f) + eps);
 }
 
-__device__ __forceinline__ void rotate16(float (&x)[16], const float* cs) {
+__device__ __forceinline__ void scale16(float (&x)[16], float r, const float (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = x[e] * r * w[e];
+}
+
+// cs: the lane's cos entries, then its sin entries.
+__device__ __forceinline__ void rotate16(float (&x)[16], const float (&cs)[16]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float a = x[e], b = x[8 + e], co = cs[e], si = cs[64 + e];
-    x[e] = __fsub_rn(__fmul_rn(a, co), __fmul_rn(b, si));
-    x[8 + e] = __fadd_rn(__fmul_rn(b, co), __fmul_rn(a, si));
+    const float a = x[e], b = x[8 + e];
+    x[e] = __builtin_fmaf(a, cs[e], -(b * cs[8 + e]));
+    x[8 + e] = __builtin_fmaf(b, cs[e], a * cs[8 + e]);
   }
 }
 
-// Query heads, eight lanes each.
+__device__ __forceinline__ void load_angles(const float* at, float (&cs)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(at + (i < 2 ? 4 * i : 64 + 4 * (i - 2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cs[4 * i + e] = v[e];
+  }
+}
+
+// Query heads: eight lanes take kQHeads heads of one row, which share the
+// row's angles (512 bytes, as much as two heads).
+constexpr int kQHeads = 4;
+
 template <bool BF16, Kv8Form FORM>
 __device__ __forceinline__ void kv8_query(const Kv8Args& a, int64_t unit, int c) {
-  if (unit >= (int64_t)a.rows * a.hq) return;  // whole groups of eight lanes
-  const int64_t row = unit / a.hq;
-  const int head = (int)(unit - row * a.hq);
-  const uint16_t* src = a.q + row * a.q_stride + (int64_t)head * 128;
-  uint16_t* dst = a.q_out + unit * 128;
+  const int groups = (a.hq + kQHeads - 1) / kQHeads;
+  const int64_t units = (int64_t)a.rows * groups;
+  if (unit >= units) return;  // whole groups of eight lanes
+  const int64_t row = units <= UINT32_MAX ? (int64_t)((uint32_t)unit / (uint32_t)groups) : unit / groups;
+  const int head = (int)(unit - row * groups) * kQHeads;
+  const uint16_t* src = a.q + row * a.q_stride + (int64_t)head * 128 + 8 * c;
+  uint16_t* dst = a.q_out + (row * a.hq + head) * 128 + 8 * c;
   const int64_t p = a.pos[row];
   const bool rot = p >= 0 && p < a.max_pos;
-  const float* cs = a.table + (rot ? p : 0) * 128 + 8 * c;
-  u32x4 lo = ldv(src + 8 * c), hi = ldv(src + 64 + 8 * c);
+  const float* at = a.table + (rot ? p : 0) * 128 + 8 * c;
+  u32x4 lo[kQHeads], hi[kQHeads];
+#pragma unroll
+  for (int i = 0; i < kQHeads; ++i) {
+    const int h = head + i < a.hq ? 128 * i : 0;
+    lo[i] = ldv(src + h);
+    hi[i] = ldv(src + h + 64);
+  }
   if constexpr (FORM == Kv8Form::Rope) {
     if (!rot) return;  // in place
-    rotate8<BF16>(lo, hi, cs, cs + 64);
-  } else {
-    float x[16];
-    unpack16<BF16>(lo, hi, x);
-    normalize16<BF16>(x, a.qw, c, a.eps);
-    if (rot) rotate16(x, cs);
-    float l[8], h[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      l[e] = x[e];
-      h[e] = x[8 + e];
+    for (int i = 0; i < kQHeads; ++i) rotate8<BF16>(lo[i], hi[i], at, at + 64);
+  } else {
+    float cs[16], w[16];
+    load_angles(at, cs);
+    unpack16<BF16>(ldv(a.qw + 8 * c), ldv(a.qw + 64 + 8 * c), w);
+#pragma unroll
+    for (int i = 0; i < kQHeads; ++i) {
+      float x[16];
+      unpack16<BF16>(lo[i], hi[i], x);
+      scale16(x, rms16(x, a.eps), w);
+      if (rot) rotate16(x, cs);
+      float l[8], h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        l[e] = x[e];
+        h[e] = x[8 + e];
+      }
+      lo[i] = pack8_rne<BF16>(l);
+      hi[i] = pack8_rne<BF16>(h);
     }
-    lo = pack8_rne<BF16>(l);
-    hi = pack8_rne<BF16>(h);
   }
-  stv(dst + 8 * c, lo);
-  stv(dst + 64 + 8 * c, hi);
+#pragma unroll
+  for (int i = 0; i < kQHeads; ++i)
+    if (head + i < a.hq) {
+      stv(dst + 128 * i, lo[i]);
+      stv(dst + 128 * i + 64, hi[i]);
+    }
 }
 
 // One wavefront takes a window of 16 rows and one (kv head, K or V).  The rows
@@ -181,9 +219,17 @@ __device__ __forceinline__ void kv8_window(const Kv8Args& a, int64_t unit) {
   for (int s = 0; s < kPasses; ++s) {
     if (((members >> (1 + 8 * s)) & 0xff) == 0) continue;
     if (FORM != Kv8Form::Store && side == 0) {
-      if constexpr (FORM == Kv8Form::NormRope) normalize16<BF16>(x[s], a.kw, c, a.eps);
+      if constexpr (FORM == Kv8Form::NormRope) {
+        float w[16];
+        unpack16<BF16>(ldv(a.kw + 8 * c), ldv(a.kw + 64 + 8 * c), w);
+        scale16(x[s], rms16(x[s], a.eps), w);
+      }
       const int at = __shfl(p, 1 + 8 * s + g, 64);
-      if (at >= 0) rotate16(x[s], a.table + (int64_t)at * 128 + 8 * c);
+      if (at >= 0) {
+        float cs[16];
+        load_angles(a.table + (int64_t)at * 128 + 8 * c, cs);
+        rotate16(x[s], cs);
+      }
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -289,7 +335,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a) {
 template <Kv8Form FORM>
 static hipError_t kv8_launch(const Kv8Args& a, bool bf16, hipStream_t st) {
   const int64_t n_kv = ((int64_t)a.rows + 15) / 16 * (2 * a.hkv);
-  const int64_t n_q = FORM == Kv8Form::Store ? 0 : ((int64_t)a.rows * a.hq + 7) / 8;
+  const int64_t n_q = FORM == Kv8Form::Store ? 0 : ((int64_t)a.rows * ((a.hq + kQHeads - 1) / kQHeads) + 7) / 8;
   const int64_t grid = (n_kv + n_q + 3) / 4;
   if (grid == 0) return hipSuccess;
   if (grid > INT32_MAX) return hipErrorInvalidValue;
@@ -365,9 +411,9 @@ hipError_t launch_norm_rope_append_kv8(const void* qkv, int64_t row_stride, cons
   return kv8_launch<Kv8Form::NormRope>(a, bf16, st);
 }
 
-// Tokens of the cache as 16-bit rows: a thread takes 16 codes of K and of V
-// (16-byte loads, two 16-byte stores each).  Rows whose slot is outside the
-// cache are left as they are.
+// Tokens of the cache as 16-bit rows: a thread takes 8 codes of K and of V, so
+// that both the loads (8 bytes) and the stores (16 bytes) of a wavefront are
+// contiguous.  Rows whose slot is outside the cache are left as they are.
 template <bool BF16>
 __global__ __launch_bounds__(256) void kv8_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                        const float* __restrict__ scales,
@@ -376,27 +422,23 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(const uint8_t* __restrict
                                                        int cache_slots) {
   const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (idx >= total) return;
-  const int64_t unit = idx >> 3;  // (row, head)
-  const int c = (int)(idx & 7);
+  const int64_t unit = idx >> 4;  // (row, head)
+  const int c = (int)(idx & 15);
   const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)unit / (uint32_t)hkv) : unit / hkv;
   const int head = (int)(unit - row * hkv);
   const int64_t slot = slots[row];
   if (slot < 0 || slot >= cache_slots) return;
-  const int64_t from = (slot * hkv + head) * 128 + 16 * c;
-  const u32x4 kw = *reinterpret_cast<const u32x4*>(kc + from);
-  const u32x4 vw = *reinterpret_cast<const u32x4*>(vc + from);
-  const float* s = scales + ((slot >> 4) * hkv + head) * 2;
-  const float ks = s[0], vs = s[1];
-  const int64_t to = unit * 128 + 16 * c;
-  stv(k_out + to, kv8_decode8<BF16>(kw[0], kw[1], ks, ks));
-  stv(k_out + to + 8, kv8_decode8<BF16>(kw[2], kw[3], ks, ks));
-  stv(v_out + to, kv8_decode8<BF16>(vw[0], vw[1], vs, vs));
-  stv(v_out + to + 8, kv8_decode8<BF16>(vw[2], vw[3], vs, vs));
+  const int64_t from = (slot * hkv + head) * 128 + 8 * c;
+  const u32x2 kw = *reinterpret_cast<const u32x2*>(kc + from);
+  const u32x2 vw = *reinterpret_cast<const u32x2*>(vc + from);
+  const f32x2 s = *reinterpret_cast<const f32x2*>(scales + ((slot >> 4) * hkv + head) * 2);
+  stv(k_out + 8 * idx, kv8_decode8<BF16>(kw[0], kw[1], s[0], s[0]));
+  stv(v_out + 8 * idx, kv8_decode8<BF16>(vw[0], vw[1], s[1], s[1]));
 }
 
 hipError_t launch_load_kv8(const void* kc, const void* vc, const float* scales, const int64_t* slots, void* k_out,
                            void* v_out, int rows, int hkv, bool bf16, int cache_slots, hipStream_t st) {
-  const int64_t total = (int64_t)rows * hkv * 8;
+  const int64_t total = (int64_t)rows * hkv * 16;
   if (total == 0) return hipSuccess;
   const int64_t grid = (total + 255) / 256;
   if (grid > INT32_MAX) return hipErrorInvalidValue;

@@ -174,11 +174,22 @@ def _i32(values: Sequence[int]):
     return arr
 
 
-def _stream(stream) -> int:
+def _current_stream() -> int:
+    """The current HIP stream.  Without the Stream object that
+    torch.cuda.current_stream() makes, which costs as much as a launch."""
     import torch
 
-    if stream is None:
+    raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+    if raw is None or device is None:
         return torch.cuda.current_stream().cuda_stream
+    torch.cuda.init()
+    globals()["_current_stream"] = lambda: raw(device())
+    return raw(device())
+
+
+def _stream(stream) -> int:
+    if stream is None:
+        return _current_stream()
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
