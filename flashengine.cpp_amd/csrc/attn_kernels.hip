@@ -732,11 +732,11 @@ __device__ __forceinline__ MergeRow ldc_merge(const MergeRow* rows, int i) {
   return MergeRow{ldc(p, 0), ldc(p, 1), ldc(p, 2), ldc(p, 3)};
 }
 
-template <bool BF16, int BATCH>
+template <bool BF16, bool SCALED, int BATCH>
 __device__ __forceinline__ void merge_fold(const MergeArgs& a, const MergeRow& mr, int head, int d, int sp0,
                                            MergeState& s) {
   size_t slot[BATCH];
-  float l[BATCH];
+  float l[BATCH], f[BATCH];
   u32x2 rv[BATCH];  // four 16-bit partial values
   // Past the last split the loads repeat it (a cache hit); what they brought
   // is replaced by zero with weight zero (a repeated infinity times zero would
@@ -750,6 +750,7 @@ __device__ __forceinline__ void merge_fold(const MergeArgs& a, const MergeRow& m
   for (int u = 0; u < BATCH; ++u) {
     slot[u] = (size_t)(mr.part + min(sp0 + u, mr.nsplit - 1) * mr.stride) * a.hq + head;
     l[u] = a.part_lse[slot[u]];
+    if constexpr (SCALED) f[u] = a.part_scale[slot[u]];
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -772,10 +773,10 @@ __device__ __forceinline__ void merge_fold(const MergeArgs& a, const MergeRow& m
 #pragma unroll
   for (int u = 0; u < BATCH; ++u) {
     rv[u] &= sp0 + u < mr.nsplit ? ~0u : 0u;
-    const f32x4 v = {lo_f32<BF16>(rv[u][0]), hi_f32<BF16>(rv[u][0]), lo_f32<BF16>(rv[u][1]),
-                     hi_f32<BF16>(rv[u][1])};
+    constexpr bool B = BF16 && !SCALED;
+    const f32x4 v = {lo_f32<B>(rv[u][0]), hi_f32<B>(rv[u][0]), lo_f32<B>(rv[u][1]), hi_f32<B>(rv[u][1])};
     s.wsum += l[u];
-    s.acc += l[u] * v;
+    s.acc += (SCALED ? l[u] * f[u] : l[u]) * v;
   }
   s.m = bm;
 }
@@ -793,7 +794,9 @@ __device__ __forceinline__ void merge_write(const MergeArgs& a, int row, int hea
 // header names; an eager launch is handed the list and its length.
 enum class MergeForm { Narrow, Wide, Header };
 
-template <bool BF16, MergeForm FORM>
+// SCALED: rows of the 8-bit caches' kernels, fp16 under a power of two of their
+// own (part_store, kv8.hpp).
+template <bool BF16, MergeForm FORM, bool SCALED>
 __global__ __launch_bounds__(256) void attn_merge_kernel(MergeArgs a) {
   constexpr int WAVES = 4, kFew = 4, kNarrow = 8, kWide = 16;
   const int lane = threadIdx.x & 63;
@@ -816,9 +819,9 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(MergeArgs a) {
       const int hh = h < a.hq ? h : a.hq - 1;
       MergeState s{kNegInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
       if (mr.nsplit <= kFew) {
-        merge_fold<BF16, kFew>(a, mr, hh, d, 0, s);
+        merge_fold<BF16, SCALED, kFew>(a, mr, hh, d, 0, s);
       } else {
-        for (int sp0 = 0; sp0 < mr.nsplit; sp0 += kNarrow) merge_fold<BF16, kNarrow>(a, mr, hh, d, sp0, s);
+        for (int sp0 = 0; sp0 < mr.nsplit; sp0 += kNarrow) merge_fold<BF16, SCALED, kNarrow>(a, mr, hh, d, sp0, s);
       }
       if (h < a.hq) merge_write<BF16>(a, mr.row, h, d, s);
     }
@@ -832,7 +835,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(MergeArgs a) {
     const int h = 2 * (pair % hpairs) + (lane >> 5);
     MergeState s{kNegInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
     for (int sp0 = kWide * wave; sp0 < mr.nsplit; sp0 += kWide * WAVES)
-      merge_fold<BF16, kWide>(a, mr, h < a.hq ? h : a.hq - 1, d, sp0, s);
+      merge_fold<BF16, SCALED, kWide>(a, mr, h < a.hq ? h : a.hq - 1, d, sp0, s);
     sh_acc[wave][lane] = s.acc;
     if (d == 0) {
       sh_m[wave][lane >> 5] = s.m;
@@ -955,19 +958,19 @@ hipError_t launch_stage_copy(void* dst, const void* src, size_t bytes, hipStream
   return hipGetLastError();
 }
 
-template <bool BF16>
+template <bool BF16, bool SCALED>
 static void merge_launch(const MergeArgs& a, int grid, hipStream_t st) {
   if (a.count_base != nullptr)
-    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Header>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Header, SCALED>), dim3(grid), dim3(256), 0, st, a);
   else if (a.wide)
-    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Wide>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Wide, SCALED>), dim3(grid), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Narrow>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Narrow, SCALED>), dim3(grid), dim3(256), 0, st, a);
 }
 
 hipError_t launch_merge(const MergeArgs& a, bool bf16, int grid, hipStream_t st) {
-  if (bf16) merge_launch<true>(a, grid, st);
-  else merge_launch<false>(a, grid, st);
+  if (a.part_scale != nullptr) bf16 ? merge_launch<true, true>(a, grid, st) : merge_launch<false, true>(a, grid, st);
+  else bf16 ? merge_launch<true, false>(a, grid, st) : merge_launch<false, false>(a, grid, st);
   return hipGetLastError();
 }
 

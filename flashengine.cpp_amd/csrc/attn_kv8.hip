@@ -31,6 +31,27 @@ __device__ __forceinline__ int swz_v(int t) {
   return ((t >> 1) & 1) | (((t >> 4) & 1) << 1) | ((((t >> 2) ^ t) & 1) << 2);
 }
 
+// Probabilities as two 16-bit operands whose sum they are within 2^-17 (bf16) or
+// 2^-23 (fp16): hi rounded, lo the rest.  The decode kernels wait for memory,
+// not for the MFMA, so the second product costs them nothing, and their results
+// carry the output's rounding alone (with hi only the error was 1.4 times that).
+template <bool BF16>
+__device__ __forceinline__ void pack2_split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<BF16>(a, b);
+  lo = pack2<BF16>(a - lo_f32<BF16>(hi), b - hi_f32<BF16>(hi));
+}
+
+template <bool BF16>
+__device__ __forceinline__ void pack8_split(const float (&x)[4], const float (&y)[4], u32x4& hi, u32x4& lo) {
+  uint32_t h[4], l[4];
+  pack2_split<BF16>(x[0], x[1], h[0], l[0]);
+  pack2_split<BF16>(x[2], x[3], h[1], l[1]);
+  pack2_split<BF16>(y[0], y[1], h[2], l[2]);
+  pack2_split<BF16>(y[2], y[3], h[3], l[3]);
+  hi = u32x4{h[0], h[1], h[2], h[3]};
+  lo = u32x4{l[0], l[1], l[2], l[3]};
+}
+
 // V^T operand of a 32-token step: lane 16 J + L of the read for dim block db
 // points at 8 bytes (dims 16 db + 8 m ..) of row k's token, L = 2 k + m: tokens
 // 4 J + k of the first 16 (k < 4) and 4 J + k - 4 of the second, the tokens
@@ -40,6 +61,71 @@ __device__ __forceinline__ void v_operand_addr(int J, int L, uint32_t (&v_lds)[8
   const int t = k < 4 ? 4 * J + k : 16 + 4 * J + k - 4;
 #pragma unroll
   for (int db = 0; db < 8; ++db) v_lds[db] = (uint32_t)(128 * t + 16 * (db ^ swz_v(t)) + 8 * m);
+}
+
+// A column's results (lane 16 J + L: dims 16 db + 4 J + r): to `out` and `lse`,
+// or to partial row `slot` when the row is split.
+template <bool BF16>
+__device__ __forceinline__ void put_column(const AttnArgs& a, const f32x4 (&o)[8], float ls, float m, int part,
+                                           int row, int slot, int head, int J) {
+  const float inv = ls > 0.f ? 1.f / ls : 0.f;
+  const float l2 = ls > 0.f ? m + __log2f(ls) : kNegInf;
+  if (part < 0) {
+    const size_t oi = (size_t)row * a.hq + head;
+    uint16_t* op = a.out + oi * kHeadDim + 4 * J;
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+      *reinterpret_cast<u32x2*>(op + 16 * db) =
+          u32x2{pack2<BF16>(o[db][0] * inv, o[db][1] * inv), pack2<BF16>(o[db][2] * inv, o[db][3] * inv)};
+    if (a.lse != nullptr && J == 0) a.lse[oi] = l2 * kLn2;
+    return;
+  }
+  float mx = 0.f;
+#pragma unroll
+  for (int db = 0; db < 8; ++db)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, fabsf(o[db][r]));
+  mx = max_x32(max_x16(mx)) * inv;
+  float is;
+  const float sc = part_scale_of(mx, is);
+  const size_t oi = (size_t)slot * a.hq + head;
+  uint16_t* op = a.part_o + oi * kHeadDim + 4 * J;
+#pragma unroll
+  for (int db = 0; db < 8; ++db)
+    *reinterpret_cast<u32x2*>(op + 16 * db) = u32x2{pack2<false>(o[db][0] * inv * is, o[db][1] * inv * is),
+                                                    pack2<false>(o[db][2] * inv * is, o[db][3] * inv * is)};
+  if (J == 0) {
+    a.part_lse[oi] = l2;
+    a.part_scale[oi] = sc;
+  }
+}
+
+// The same for a combined column that 32 lanes hold (lane c: dims 4 c .. + 3).
+template <bool BF16>
+__device__ __forceinline__ void put_combined(const AttnArgs& a, f32x4 acc, float ls, float top, int part, int row,
+                                             int slot, int head, int c) {
+  const float inv = ls > 0.f ? 1.f / ls : 0.f;
+  const float l2 = ls > 0.f ? top + __log2f(ls) : kNegInf;
+  acc *= inv;
+  if (part < 0) {
+    const size_t oi = (size_t)row * a.hq + head;
+    *reinterpret_cast<u32x2*>(a.out + oi * kHeadDim + 4 * c) =
+        u32x2{pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3])};
+    if (a.lse != nullptr && c == 0) a.lse[oi] = l2 * kLn2;
+    return;
+  }
+  float mx = fmaxf(fmaxf(fabsf(acc[0]), fabsf(acc[1])), fmaxf(fabsf(acc[2]), fabsf(acc[3])));
+#pragma unroll
+  for (int d = 1; d <= 16; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+  float is;
+  const float sc = part_scale_of(mx, is);
+  const size_t oi = (size_t)slot * a.hq + head;
+  *reinterpret_cast<u32x2*>(a.part_o + oi * kHeadDim + 4 * c) =
+      u32x2{pack2<false>(acc[0] * is, acc[1] * is), pack2<false>(acc[2] * is, acc[3] * is)};
+  if (c == 0) {
+    a.part_lse[oi] = l2;
+    a.part_scale[oi] = sc;
+  }
 }
 
 // ===========================================================================
@@ -218,7 +304,7 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
           load_k();  // under the softmax
         }
 
-        u32x4 pf[2][NCB];
+        u32x4 pf[2][NCB], pl[2][NCB];
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
           float mx = kNegInf;
@@ -250,10 +336,7 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
             for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
           }
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-            pf[ks][cb] = u32x4{pack2<BF16>(x[2 * ks][0], x[2 * ks][1]), pack2<BF16>(x[2 * ks][2], x[2 * ks][3]),
-                               pack2<BF16>(x[2 * ks + 1][0], x[2 * ks + 1][1]),
-                               pack2<BF16>(x[2 * ks + 1][2], x[2 * ks + 1][3])};
+          for (int ks = 0; ks < 2; ++ks) pack8_split<BF16>(x[2 * ks], x[2 * ks + 1], pf[ks][cb], pl[ks][cb]);
         }
 
         __builtin_amdgcn_sched_barrier(0);
@@ -273,6 +356,8 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
               const u32x4 vf = kv8_decode8<BF16>(w[0], w[1], sv[2 * ks][1], sv[2 * ks + 1][1]);
 #pragma unroll
               for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[ks][cb], o[db][cb]);
+#pragma unroll
+              for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pl[ks][cb], o[db][cb]);
             }
           }
         if (more) {
@@ -330,19 +415,8 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
           ls += lw[w] * wt;
           acc += *(lds_f32x4*)(uintptr_t)(lbase + (uint32_t)(w * kShort8Wave + 512 * n + 16 * (c ^ (n & 15)))) * wt;
         }
-      const float inv = ls > 0.f ? 1.f / ls : 0.f;
-      const float l2 = ls > 0.f ? top + __log2f(ls) : kNegInf;
       const int r = n / G, head = kvh * G + (n - r * G);
-      const u32x2 v = {pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
-      if (part < 0) {
-        const size_t oi = (size_t)(q0 + r) * a.hq + head;
-        *reinterpret_cast<u32x2*>(a.out + oi * kHeadDim + 4 * c) = v;
-        if (a.lse != nullptr && c == 0) a.lse[oi] = l2 * kLn2;
-      } else {
-        const size_t oi = (size_t)(part + r) * a.hq + head;
-        *reinterpret_cast<u32x2*>(a.part_o + oi * kHeadDim + 4 * c) = v;
-        if (c == 0) a.part_lse[oi] = l2;
-      }
+      put_combined<BF16>(a, acc, ls, top, part, q0 + r, part + r, head, c);
     }
     if constexpr (GRID2) break;
     if (it + (int)gridDim.x < n_items) __syncthreads();  // the regions are the next item's V
@@ -583,7 +657,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
         }
       }
 
-      u32x4 pf[NCB];
+      u32x4 pf[NCB], pl[NCB];
       float alpha[NCB];
       bool any_up = false;
 #pragma unroll
@@ -614,8 +688,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
             ps += x[tb][r];
           }
         lsum[cb] = lsum[cb] * alpha[cb] + ps;
-        pf[cb] = u32x4{pack2<BF16>(x[0][0], x[0][1]), pack2<BF16>(x[0][2], x[0][3]), pack2<BF16>(x[1][0], x[1][1]),
-                       pack2<BF16>(x[1][2], x[1][3])};
+        pack8_split<BF16>(x[0], x[1], pf[cb], pl[cb]);
       }
 
       if (t1 - tok < 32) {
@@ -641,6 +714,8 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
         const u32x4 vf = kv8_decode8<BF16>(vw[db][0], vw[db][1], vs[0], vs[1]);
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[cb], o[db][cb]);
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pl[cb], o[db][cb]);
       }
       consumed += 2;
       r_slot = v_slot + 1 == U ? 0 : v_slot + 1;
@@ -650,22 +725,10 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
     for (int cb = 0; cb < NCB; ++cb) {
       const float ls = sum_x32(sum_x16(lsum[cb]));
       if (col_ok[cb]) {
-        const float inv = ls > 0.f ? 1.f / ls : 0.f;
-        const float l2 = ls > 0.f ? m[cb] + __log2f(ls) : kNegInf;
-        const bool whole = w.part < 0;
-        const size_t oi = whole ? (size_t)crow[cb] * a.hq + chead[cb]
-                                : (size_t)(w.part + (16 * cb + L) / G) * a.hq + chead[cb];
-        uint16_t* op = (whole ? a.out : a.part_o) + oi * kHeadDim + 4 * J;
+        f32x4 oc[8];
 #pragma unroll
-        for (int db = 0; db < 8; ++db) {
-          const u32x2 v = {pack2<BF16>(o[db][cb][0] * inv, o[db][cb][1] * inv),
-                           pack2<BF16>(o[db][cb][2] * inv, o[db][cb][3] * inv)};
-          *reinterpret_cast<u32x2*>(op + 16 * db) = v;
-        }
-        if (J == 0) {
-          if (!whole) a.part_lse[oi] = l2;
-          else if (a.lse != nullptr) a.lse[oi] = l2 * kLn2;
-        }
+        for (int db = 0; db < 8; ++db) oc[db] = o[db][cb];
+        put_column<BF16>(a, oc, ls, m[cb], w.part, crow[cb], w.part + (16 * cb + L) / G, chead[cb], J);
       }
     }
   }
@@ -907,21 +970,10 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
       const float ln = sum_x32(sum_x16(lsum[cb]));
       const int n = wave * kWcols + 16 * cb + L;
       if (n < ncols) {
-        const float inv = ln > 0.f ? 1.f / ln : 0.f;
-        const float l2 = ln > 0.f ? m[cb] + __log2f(ln) : kNegInf;
-        const bool whole = w.part < 0;
-        const size_t oi = whole ? (size_t)crow[cb] * a.hq + chead[cb] : (size_t)(w.part + n / G) * a.hq + chead[cb];
-        uint16_t* op = (whole ? a.out : a.part_o) + oi * kHeadDim + 4 * J;
+        f32x4 oc[8];
 #pragma unroll
-        for (int db = 0; db < 8; ++db) {
-          const u32x2 v = {pack2<BF16>(o[db][cb][0] * inv, o[db][cb][1] * inv),
-                           pack2<BF16>(o[db][cb][2] * inv, o[db][cb][3] * inv)};
-          *reinterpret_cast<u32x2*>(op + 16 * db) = v;
-        }
-        if (J == 0) {
-          if (!whole) a.part_lse[oi] = l2;
-          else if (a.lse != nullptr) a.lse[oi] = l2 * kLn2;
-        }
+        for (int db = 0; db < 8; ++db) oc[db] = o[db][cb];
+        put_column<BF16>(a, oc, ln, m[cb], w.part, crow[cb], w.part + n / G, chead[cb], J);
       }
     }
   }
@@ -957,7 +1009,6 @@ __device__ __forceinline__ void block8_item(const AttnArgs& a, const WorkItem& w
   const int pmask = (1 << pshift) - 1;
   const int row_bytes = a.hkv * kHeadDim;
   const uint32_t ring = lbase + (uint32_t)(kBlk8Q + wave * kBlk8Wave);
-  typedef __attribute__((address_space(3))) float lds_f32;
   typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
@@ -1233,17 +1284,8 @@ __device__ __forceinline__ void block8_item(const AttnArgs& a, const WorkItem& w
           ls += st[v][1] * wt;
           acc += *(lds_f32x4*)(uintptr_t)(lbase + (uint32_t)(16384 * v + 512 * n + 16 * (c ^ (n & 15)))) * wt;
         }
-        const float inv = ls > 0.f ? 1.f / ls : 0.f;
-        const float l2 = ls > 0.f ? top + __log2f(ls) : kNegInf;
         const int r = col / G, head = kvh * G + (col - r * G);
-        const bool whole = w.part < 0;
-        const size_t oi = (size_t)(whole ? w.q0 + r : w.part + r) * a.hq + head;
-        const u32x2 v2 = {pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
-        *reinterpret_cast<u32x2*>((whole ? a.out : a.part_o) + oi * kHeadDim + 4 * c) = v2;
-        if (c == 0) {
-          if (!whole) a.part_lse[oi] = l2;
-          else if (a.lse != nullptr) a.lse[oi] = l2 * kLn2;
-        }
+        put_combined<BF16>(a, acc, ls, top, w.part, w.q0 + r, w.part + r, head, c);
       }
     }
   }

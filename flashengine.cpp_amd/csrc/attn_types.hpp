@@ -131,6 +131,7 @@ struct AttnArgs {
   int group;               // hq / hkv
   int page_shift;          // log2(page)
   float scale_log2;        // log2(e) / sqrt(128)
+  float* part_scale;       // 8-bit caches: [slots][hq] powers of two that the partial rows are held under
   const float* scales;     // 8-bit caches: [16-token block][hkv][2] powers of two (kc, vc then hold e4m3 codes)
 };
 
@@ -143,6 +144,7 @@ struct MergeArgs {
   const int32_t* count_base;  // graph launches, device-resident: records to fold, index of the first in `rows`, wide
   const uint16_t* part_o;
   const float* part_lse;
+  const float* part_scale;    // null: rows in the attention's type; else fp16 rows, to be scaled by these
   int hq;
 };
 

@@ -326,6 +326,7 @@ struct Launch {
   const uint8_t* dev = nullptr;  // metadata arena on the device
   uint16_t* part_o = nullptr;    // 16-bit split-KV partial rows
   float* part_lse = nullptr;
+  float* part_scale = nullptr;   // the partial rows' powers of two (8-bit caches)
   bool bf16 = true;
   bool graph = false;
   int graph_tile = -1;  // graph plans: the first graph prepare had tile work (1) or not (0)
@@ -502,6 +503,7 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
   a.page_shift = shift;
   a.scale_log2 = 1.4426950408889634f / 11.313708498984761f;  // log2(e) / sqrt(128)
   a.scales = scales;
+  a.part_scale = L.part_scale;
   hipError_t e;
   if (L.graph || L.n_decode > 0 || L.n_short > 0) {
     AttnArgs d = a;
@@ -542,6 +544,7 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
     }
     m.part_o = L.part_o;
     m.part_lse = L.part_lse;
+    m.part_scale = scales != nullptr ? L.part_scale : nullptr;
     m.hq = L.sh.hq;
     m.wide = L.wide_merge[mode] ? 1 : 0;
     e = launch_merge(m, L.bf16, merge_grid(L, mode), st);
@@ -702,7 +705,8 @@ int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int m
     return cleanup(FE_EDEVICE, "hipHostGetDevicePointer(plan staging) failed");
   if (hipMalloc(&p->part_o, (size_t)sh.partial_cap * hq * kHeadDim * sizeof(uint16_t)) != hipSuccess)
     return cleanup(FE_ENOMEM, "hipMalloc(split-KV partials) failed");
-  if (hipMalloc(&p->part_lse, (size_t)sh.partial_cap * hq * sizeof(float)) != hipSuccess)
+  // the log-sum-exps, and behind them the rows' scales (8-bit caches)
+  if (hipMalloc(&p->part_lse, 2 * (size_t)sh.partial_cap * hq * sizeof(float)) != hipSuccess)
     return cleanup(FE_ENOMEM, "hipMalloc(split-KV lse) failed");
   if (hipEventCreateWithFlags(&p->staged, hipEventDisableTiming) != hipSuccess)
     return cleanup(FE_EDEVICE, "hipEventCreate failed");
@@ -712,6 +716,7 @@ int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int m
   p->run.dev = p->dev;
   p->run.part_o = p->part_o;
   p->run.part_lse = p->part_lse;
+  p->run.part_scale = p->part_lse + (size_t)sh.partial_cap * hq;
   *plan_out = p;
   return FE_OK;
 }

@@ -159,6 +159,58 @@ __device__ __forceinline__ void kv8_query(const Kv8Args& a, int64_t unit, int c)
     }
 }
 
+// Keys are computed in 64 bits and rounded to their codes once: a code has so
+// few bits that an error of 2^-24 before its rounding shows as a whole step of
+// an element now and then, where other elements show nothing.  Queries need
+// no such care, and keys are a small part of a call (8192 rows of 32/8 heads:
+// no time).  What kv8_encode4 is given is the 64-bit value rounded to odd, from
+// which the rounding to a code is that of the value itself.
+__device__ __forceinline__ float round_odd(double d) {
+  const float f = (float)d;
+  uint32_t u = __float_as_uint(f);
+  const double back = (double)f;
+  if (fabs(back) > fabs(d)) --u;          // towards zero
+  if (back != d) u |= 1u;                 // and the rest as a last bit
+  return f == f && fabsf(f) < __builtin_huge_valf() ? __uint_as_float(u) : f;
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)dpp_bits<CTRL>((uint32_t)b) | (uint64_t)dpp_bits<CTRL>((uint32_t)(b >> 32)) << 32);
+}
+
+// x: the lane's 16 elements of a key; w, cs: weights and angles, where used.
+template <bool NORM>
+__device__ __forceinline__ void key16(float (&x)[16], const float (&w)[16], float eps, bool rot, const float (&cs)[16]) {
+  double d[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) d[e] = (double)x[e];
+  if constexpr (NORM) {
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s = __builtin_fma(d[e], d[e], s);
+    s += dpp64<kXor1>(s);
+    s += dpp64<kXor2>(s);
+    s += dpp64<kHalfMirror>(s);
+    s = s * (1.0 / 128.0) + (double)eps;
+    double r = __builtin_amdgcn_rsq(s);  // good to some 2^-23: one step of Newton's iteration
+    r *= 1.5 - 0.5 * s * r * r;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) d[e] *= r * (double)w[e];
+  }
+  if (rot) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const double a = d[e], b = d[8 + e], c = (double)cs[e], n = (double)cs[8 + e];
+      d[e] = __builtin_fma(a, c, -(b * n));
+      d[8 + e] = __builtin_fma(b, c, a * n);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = round_odd(d[e]);
+}
+
 // One wavefront takes a window of 16 rows and one (kv head, K or V).  The rows
 // of a call that go to one scale block follow one another; such a run belongs
 // to the window its first row lies in, whose wavefront sees all of its values
@@ -219,17 +271,11 @@ __device__ __forceinline__ void kv8_window(const Kv8Args& a, int64_t unit) {
   for (int s = 0; s < kPasses; ++s) {
     if (((members >> (1 + 8 * s)) & 0xff) == 0) continue;
     if (FORM != Kv8Form::Store && side == 0) {
-      if constexpr (FORM == Kv8Form::NormRope) {
-        float w[16];
-        unpack16<BF16>(ldv(a.kw + 8 * c), ldv(a.kw + 64 + 8 * c), w);
-        scale16(x[s], rms16(x[s], a.eps), w);
-      }
       const int at = __shfl(p, 1 + 8 * s + g, 64);
-      if (at >= 0) {
-        float cs[16];
-        load_angles(a.table + (int64_t)at * 128 + 8 * c, cs);
-        rotate16(x[s], cs);
-      }
+      float w[16] = {}, cs[16];
+      if constexpr (FORM == Kv8Form::NormRope) unpack16<BF16>(ldv(a.kw + 8 * c), ldv(a.kw + 64 + 8 * c), w);
+      load_angles(a.table + (int64_t)max(at, 0) * 128 + 8 * c, cs);
+      key16<FORM == Kv8Form::NormRope>(x[s], w, a.eps, at >= 0, cs);
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
