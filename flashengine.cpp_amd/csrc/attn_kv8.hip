@@ -583,6 +583,10 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
     wait_lds();
     while (c_live && issued - consumed < U) issue_one();
   };
+  auto refill_after_reads = [&]() {  // the unit read last is done with
+    consumed += 1;
+    refill();
+  };
   typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 
   for (int it = it_begin; it < it_end; ++it) {
@@ -633,43 +637,43 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
       // so that each page is requested by all of them at about the same time.
       if (((tok - t0) & 32) == 0) __builtin_amdgcn_s_barrier();
       refill();
-      wait_units<U, 5>(issued - consumed - 2);
+      // ---- S^T; the K unit's slot is refilled as soon as it is read
+      wait_units<U, 5>(issued - consumed - 1);
       const uint32_t kst = ring + (uint32_t)(r_slot * kKv8Slot);
-      const int v_slot = r_slot + 1 == U ? 0 : r_slot + 1;
-      const uint32_t vst = ring + (uint32_t)(v_slot * kKv8Slot);
-
+      r_slot = r_slot + 1 == U ? 0 : r_slot + 1;
       const f32x2 ks = *(lds_f32x2*)(uintptr_t)(kst + kKv8Unit);
-      const f32x2 vs = *(lds_f32x2*)(uintptr_t)(vst + kKv8Unit);
+      u32x4 kw[2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) kw[tb][s] = lds_read16(kst + 2048 * tb + k_lds[s]);
+      refill_after_reads();
       f32x4 sc[2][NCB];
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const u32x4 kw = lds_read16(kst + 2048 * tb + k_lds[s]);
+        for (int k = 0; k < 4; ++k) {
+          const u32x4 kf = kv8_decode8<BF16>(kw[tb][k >> 1][2 * (k & 1)], kw[tb][k >> 1][2 * (k & 1) + 1], ks[tb], ks[tb]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x4 kf = kv8_decode8<BF16>(kw[2 * h], kw[2 * h + 1], ks[tb], ks[tb]);
-#pragma unroll
-            for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = mfma16<BF16>(kf, qf[cb][2 * s + h], sc[tb][cb]);
-          }
+          for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = mfma16<BF16>(kf, qf[cb][k], sc[tb][cb]);
         }
       }
 
-      u32x4 pf[NCB], pl[NCB];
+      // ---- softmax: the statistics, then the exponentials under the reads of V
+      float x[NCB][2][4];
       float alpha[NCB];
       bool any_up = false;
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
-        float x[2][4];
         float mx = kNegInf;
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[tb][r] = tok + 16 * tb + 4 * J + r <= lim[cb] ? sc[tb][cb][r] * a.scale_log2 : kNegInf;
-            mx = fmaxf(mx, x[tb][r]);
+            x[cb][tb][r] = tok + 16 * tb + 4 * J + r <= lim[cb] ? sc[tb][cb][r] * a.scale_log2 : kNegInf;
+            mx = fmaxf(mx, x[cb][tb][r]);
           }
         mx = max_x32(max_x16(mx));
         // Lazy reference maximum: raised (with l and o rescaled) only when the
@@ -678,19 +682,19 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
         alpha[cb] = up ? fast_exp2(m[cb] - mx) : 1.f;
         if (up) m[cb] = mx;
         any_up = any_up || up;
-        const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
-        float ps = 0.f;
+      }
+      if (__builtin_amdgcn_ballot_w64(any_up) != 0) {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+        for (int cb = 0; cb < NCB; ++cb) {
+          lsum[cb] *= alpha[cb];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[tb][r] = fast_exp2(x[tb][r] - m_use);
-            ps += x[tb][r];
-          }
-        lsum[cb] = lsum[cb] * alpha[cb] + ps;
-        pack8_split<BF16>(x[0], x[1], pf[cb], pl[cb]);
+          for (int db = 0; db < 8; ++db) o[db][cb] *= alpha[cb];
+        }
       }
 
+      wait_units<U, 5>(issued - consumed - 1);
+      const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
+      r_slot = r_slot + 1 == U ? 0 : r_slot + 1;
       if (t1 - tok < 32) {
         // Rows past the item end hold stale contents: zero them, so that
         // 0 * (stale) can never become NaN.  (16-byte chunk q lies in row q / 8.)
@@ -700,15 +704,28 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
           if ((q >> 3) >= t1 - tok) lds_zero16(vst + 16 * q);
         }
       }
-      if (__builtin_amdgcn_ballot_w64(any_up) != 0) {
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-          for (int db = 0; db < 8; ++db) o[db][cb] *= alpha[cb];
-      }
+      const f32x2 vs = *(lds_f32x2*)(uintptr_t)(vst + kKv8Unit);
       u32x2 vw[8];
 #pragma unroll
       for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + v_lds[db]);
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 pf[NCB], pl[NCB];
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+        float ps = 0.f;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[cb][tb][r] = fast_exp2(x[cb][tb][r] - m_use);
+            ps += x[cb][tb][r];
+          }
+        lsum[cb] += ps;
+        pack8_split<BF16>(x[cb][0], x[cb][1], pf[cb], pl[cb]);
+      }
+
+      // ---- O^T
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
         const u32x4 vf = kv8_decode8<BF16>(vw[db][0], vw[db][1], vs[0], vs[1]);
@@ -717,8 +734,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pl[cb], o[db][cb]);
       }
-      consumed += 2;
-      r_slot = v_slot + 1 == U ? 0 : v_slot + 1;
+      consumed += 1;
     }
 
 #pragma unroll
