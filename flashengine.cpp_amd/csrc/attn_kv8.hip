@@ -31,6 +31,35 @@ __device__ __forceinline__ int swz_v(int t) {
   return ((t >> 1) & 1) | (((t >> 4) & 1) << 1) | ((((t >> 2) ^ t) & 1) << 2);
 }
 
+// Reference maximum of a column that has seen no token.  (Finite: differences
+// with it need no special case.)
+constexpr float kEmpty = -3.4028234663852886e38f;
+
+// The running reference maximum m of each column, in log2 units, is lazy: it is
+// raised, and l and o with it rescaled, only where a step's maximum exceeds it
+// by more than 8, so that p <= 2^8.  Whether any does needs no exchange between
+// the lanes of a column: each compares its own maximum mx, and the vote of the
+// wavefront stands for the rest.  (With the columns' maxima exchanged every step,
+// draft blocks took @BLOCKS@, prefill @PREFILL@.)
+template <int NCB>
+__device__ __forceinline__ void raise_max(const float (&mx)[NCB], float scale, float (&m)[NCB], float (&lsum)[NCB],
+                                          f32x4 (&o)[8][NCB]) {
+  bool above = false;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) above = above || mx[cb] * scale > m[cb] + 8.f;
+  if (__builtin_amdgcn_ballot_w64(above) == 0) return;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const float mt = max_x32(max_x16(mx[cb])) * scale;
+    const bool up = mt > m[cb] + 8.f;
+    const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
+    if (up) m[cb] = mt;
+    lsum[cb] *= alpha;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
+  }
+}
+
 // Probabilities as two 16-bit operands whose sum they are within 2^-17 (bf16) or
 // 2^-23 (fp16): hi rounded, lo the rest.  The decode kernels wait for memory,
 // not for the MFMA, so the second product costs them nothing, and their results
@@ -217,7 +246,7 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
     f32x4 o[8][NCB];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      m[cb] = kNegInf;
+      m[cb] = kEmpty;
       lsum[cb] = 0.f;
 #pragma unroll
       for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -304,37 +333,32 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
           load_k();  // under the softmax
         }
 
-        u32x4 pf[2][NCB], pl[2][NCB];
+        float mx[NCB];
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
-          float mx = kNegInf;
+          mx[cb] = kNegInf;
 #pragma unroll
           for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
-              mx = fmaxf(mx, sc[tb][cb][r]);
+              mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
             }
-          mx = max_x32(max_x16(mx));
-          const float mt = mx * a.scale_log2;
-          const bool up = mt > m[cb] + 8.f;  // lazy reference maximum, as in the tile kernel
-          const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
-          if (up) m[cb] = mt;
-          const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+        }
+        raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
+        u32x4 pf[2][NCB], pl[2][NCB];
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
           float x[4][4];
           float ps = 0.f;
 #pragma unroll
           for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m_use));
+              x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
               ps += x[tb][r];
             }
-          lsum[cb] = lsum[cb] * alpha + ps;
-          if (__builtin_amdgcn_ballot_w64(up) != 0) {
-#pragma unroll
-            for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
-          }
+          lsum[cb] += ps;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) pack8_split<BF16>(x[2 * ks], x[2 * ks + 1], pf[ks][cb], pl[ks][cb]);
         }
@@ -626,7 +650,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
     f32x4 o[8][NCB];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      m[cb] = kNegInf;
+      m[cb] = kEmpty;
       lsum[cb] = 0.f;
 #pragma unroll
       for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -662,35 +686,19 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
       }
 
       // ---- softmax: the statistics, then the exponentials under the reads of V
-      float x[NCB][2][4];
-      float alpha[NCB];
-      bool any_up = false;
+      float mx[NCB];
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
-        float mx = kNegInf;
+        mx[cb] = kNegInf;
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[cb][tb][r] = tok + 16 * tb + 4 * J + r <= lim[cb] ? sc[tb][cb][r] * a.scale_log2 : kNegInf;
-            mx = fmaxf(mx, x[cb][tb][r]);
+            if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
+            mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
           }
-        mx = max_x32(max_x16(mx));
-        // Lazy reference maximum: raised (with l and o rescaled) only when the
-        // step's maximum exceeds it by more than 8, so p <= 2^8.
-        const bool up = mx > m[cb] + 8.f;
-        alpha[cb] = up ? fast_exp2(m[cb] - mx) : 1.f;
-        if (up) m[cb] = mx;
-        any_up = any_up || up;
       }
-      if (__builtin_amdgcn_ballot_w64(any_up) != 0) {
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-          lsum[cb] *= alpha[cb];
-#pragma unroll
-          for (int db = 0; db < 8; ++db) o[db][cb] *= alpha[cb];
-        }
-      }
+      raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
 
       wait_units<U, 5>(issued - consumed - 1);
       const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
@@ -712,17 +720,17 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
       u32x4 pf[NCB], pl[NCB];
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
-        const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+        float x[2][4];
         float ps = 0.f;
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[cb][tb][r] = fast_exp2(x[cb][tb][r] - m_use);
-            ps += x[cb][tb][r];
+            x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
+            ps += x[tb][r];
           }
         lsum[cb] += ps;
-        pack8_split<BF16>(x[cb][0], x[cb][1], pf[cb], pl[cb]);
+        pack8_split<BF16>(x[0], x[1], pf[cb], pl[cb]);
       }
 
       // ---- O^T
@@ -859,7 +867,7 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
   f32x4 o[8][NCB];
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
-    m[cb] = kNegInf;
+    m[cb] = kEmpty;
     lsum[cb] = 0.f;
 #pragma unroll
     for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -883,10 +891,10 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
       }
     }
 
-    u32x4 pf[2][NCB];
+    float mx[NCB];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      float mx = kNegInf;
+      mx[cb] = kNegInf;
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
@@ -894,28 +902,23 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
           if constexpr (MASK) {
             if (T + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
           }
-          mx = fmaxf(mx, sc[tb][cb][r]);
+          mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
         }
-      mx = max_x32(max_x16(mx));
-      const float mt = mx * a.scale_log2;
-      const bool up = mt > m[cb] + 8.f;  // lazy reference maximum, p <= 2^8
-      const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
-      if (up) m[cb] = mt;
-      const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
+    }
+    raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
+    u32x4 pf[2][NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
       float x[4][4];
       float ps = 0.f;
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m_use));
+          x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
           ps += x[tb][r];
         }
-      lsum[cb] = lsum[cb] * alpha + ps;
-      if (__builtin_amdgcn_ballot_w64(up) != 0) {
-#pragma unroll
-        for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
-      }
+      lsum[cb] += ps;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
         pf[ks][cb] = u32x4{pack2<BF16>(x[2 * ks][0], x[2 * ks][1]), pack2<BF16>(x[2 * ks][2], x[2 * ks][3]),
@@ -999,32 +1002,37 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
 // ---------------------------------------------------------------------------
 // Items of at most 64 columns (draft blocks, verify rows): HBM bound
 // ---------------------------------------------------------------------------
-// Here each wavefront owns tokens instead of columns: steps of 32 tokens go to
-// the four wavefronts in turn, every wavefront computes all 64 columns on its
-// own, from codes that it alone copies, converts and reads once, with no
-// barrier from the first step to the last; the four results are combined in
-// LDS at the end of the item.  Q (64 columns, 16 KB) lies in LDS.
-constexpr int kBlk8Q = 64 * 256;
+// Here each wavefront owns tokens instead of columns: an item's steps of 32
+// tokens go to four wavefronts in turn, each computes all 64 columns on its own,
+// from codes that it alone copies, converts and reads once, with no barrier
+// inside an item.  The ring of units runs on into the next item while the four
+// results of one are combined.  Q (64 columns, 16 KB) lies in LDS, in the region
+// that combining uses in its turn.
+//
+// Two such groups of four wavefronts, neighbouring kv heads of the same tokens,
+// make a workgroup where the list is an equal cut of the tokens (pairs):
+// their reads meet in 256 bytes of a cache row.  One kv head's 128 bytes a row
+// are what such a stream reads alone, 5.8 TB/s with nothing computed against
+// 6.5 for two heads and 6.9 for four and more.
 constexpr int kBlk8Units = 3;
 constexpr int kBlk8Wave = kBlk8Units * kKv8Slot;
-constexpr int kBlk8Stats = 4 * 16384;  // combining: 32 columns x 128 fp32 of each wavefront, then the statistics
-static_assert(kBlk8Stats + 4 * 64 * 8 <= kTile8Lds && kBlk8Q + 4 * kBlk8Wave <= kTile8Lds, "");
+constexpr int kBlk8Head = kTile8Lds - 4 * kBlk8Wave;  // Q, or: exchange, then statistics
+constexpr int kBlk8Stats = 4 * 3 * 2048;  // what the wavefronts hand each other of 16 columns
+static_assert(kBlk8Head >= 64 * 256 && kBlk8Head >= kBlk8Stats + 4 * 64 * 12 && kBlk8Head % 256 == 0, "");
 
+// Items [it0, it1) of the list, by the four wavefronts (wv) that share `qbase`;
+// every wavefront of the workgroup makes the same number of calls and items.
 template <bool BF16, bool CAUSAL, bool STREAM>
-__device__ __forceinline__ void block8_item(const AttnArgs& a, const WorkItem& w, const SeqInfo& s, uint32_t lbase,
-                                            int wave, int lane) {
+__device__ __forceinline__ void block8_items(const AttnArgs& a, int it0, int it1, uint32_t qbase, uint32_t ring,
+                                             int wv, int lane) {
   constexpr int NCB = 4;
   const int J = lane >> 4;
   const int L = lane & 15;
   const int G = a.group;
-  const int kvh = w.kvh;
-  const int t0 = w.t0;
-  const int t1 = w.t1;
-  const int ncols = w.nq * G;
   const int pshift = a.page_shift;
   const int pmask = (1 << pshift) - 1;
   const int row_bytes = a.hkv * kHeadDim;
-  const uint32_t ring = lbase + (uint32_t)(kBlk8Q + wave * kBlk8Wave);
+  typedef __attribute__((address_space(3))) float lds_f32;
   typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
@@ -1049,30 +1057,31 @@ __device__ __forceinline__ void block8_item(const AttnArgs& a, const WorkItem& w
     v_at = (uint32_t)(128 * t + 16 * swz_v(t) + 8 * (L & 1));
   }
 
-  // Q: wavefront w copies column block w; columns past the item repeat its first.
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = 4 * r + J;
-    const int col = 16 * wave + n;
-    const int nn = col < ncols ? col : 0;
-    lds_dma16(a.q + ((size_t)(w.q0 + nn / G) * a.hq + kvh * G + nn % G) * kHeadDim + 8 * (L ^ n),
-              lbase + (uint32_t)(4096 * wave + 1024 * r));
-  }
-
   // ---- copy side: K, then V of this wavefront's steps (tokens c_tok .. + 31)
-  auto page_id = [&](int tok) { return ldc(a.pages, s.page_off + (tok >> pshift)); };
-  auto block_of = [&](int tok, int pg) { return ((size_t)pg << (pshift - 4)) + (size_t)((tok & pmask) >> 4); };
-  int c_tok = t0 + 32 * wave;
-  bool c_live = c_tok < t1, c_key = true;
+  // of item c_it, through the items.
+  int c_it = it0 - 1, c_tok = 0, c_t1 = 0, c_pages = 0, c_kvh = 0;
   int pg0 = 0, pg1 = 0;
-  if (c_live) {
-    pg0 = page_id(c_tok);
-    pg1 = page_id(min(c_tok + 16, t1 - 1));
-  }
+  bool c_live = true, c_key = true;
   size_t blk0 = 0, blk1 = 0;
   int issued = 0, consumed = 0, c_slot = 0, r_slot = 0;
+  auto next_item = [&]() {  // the next item with a step of this wavefront
+    while (c_tok >= c_t1) {
+      if (++c_it >= it1) {
+        c_live = false;
+        return;
+      }
+      const WorkItem n = ldc_item(a.items, c_it);
+      c_tok = n.t0 + 32 * wv;
+      c_t1 = n.t1;
+      c_kvh = n.kvh;
+      c_pages = ldc_seq(a.seqs, n.seq).page_off;
+    }
+    pg0 = ldc(a.pages, c_pages + (c_tok >> pshift));
+    pg1 = ldc(a.pages, c_pages + (min(c_tok + 16, c_t1 - 1) >> pshift));
+  };
+  auto block_of = [&](int tok, int pg) { return ((size_t)pg << (pshift - 4)) + (size_t)((tok & pmask) >> 4); };
   auto issue_codes = [&](const void* cache, const uint32_t (&goff)[4], int side, uint32_t dst) {
-    const char* base = reinterpret_cast<const char*>(cache) + (size_t)kvh * kHeadDim;
+    const char* base = reinterpret_cast<const char*>(cache) + (size_t)c_kvh * kHeadDim;
     const char* b0 = base + blk0 * (size_t)(16 * row_bytes);
     const char* b1 = base + blk1 * (size_t)(16 * row_bytes);
     lds_dma16<STREAM>(b0, goff[0], dst);
@@ -1080,238 +1089,318 @@ __device__ __forceinline__ void block8_item(const AttnArgs& a, const WorkItem& w
     lds_dma16<STREAM>(b1, goff[2], dst + 2048);
     lds_dma16<STREAM>(b1, goff[3], dst + 3072);
     const size_t at = (lane & 1) ? blk1 : blk0;
-    lds_dma4(a.scales + 2 * (at * (size_t)a.hkv + (size_t)kvh) + side, dst + kKv8Unit);
+    lds_dma4(a.scales + 2 * (at * (size_t)a.hkv + (size_t)c_kvh) + side, dst + kKv8Unit);
   };
   auto refill = [&]() {  // (the caller has waited for its reads of the slot freed last)
     while (c_live && issued - consumed < kBlk8Units) {
       const uint32_t dst = ring + (uint32_t)(c_slot * kKv8Slot);
       if (c_key) {
         blk0 = block_of(c_tok, pg0);
-        blk1 = c_tok + 16 < t1 ? block_of(c_tok + 16, pg1) : blk0;
+        blk1 = c_tok + 16 < c_t1 ? block_of(c_tok + 16, pg1) : blk0;
         const uint32_t kg[4] = {k_goff[0], k_goff[1], k_goff[0], k_goff[1]};
         issue_codes(a.kc, kg, 0, dst);
-        if (c_tok + 128 < t1) {
-          pg0 = page_id(c_tok + 128);
-          pg1 = page_id(min(c_tok + 144, t1 - 1));
+        if (c_tok + 128 < c_t1) {
+          pg0 = ldc(a.pages, c_pages + ((c_tok + 128) >> pshift));
+          pg1 = ldc(a.pages, c_pages + (min(c_tok + 144, c_t1 - 1) >> pshift));
         }
       } else {
         issue_codes(a.vc, v_goff, 1, dst);
         c_tok += 128;
-        c_live = c_tok < t1;
+        if (c_tok >= c_t1) next_item();
       }
       c_key = !c_key;
       ++issued;
       c_slot = c_slot + 1 == kBlk8Units ? 0 : c_slot + 1;
     }
   };
-  refill();
-
-  int lim[NCB];
-  int lim_min = 1 << 30;
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) {
-    const int n = 16 * cb + L;
-    lim[cb] = -1;
-    if (n < ncols) {
-      lim[cb] = min(CAUSAL ? s.len - s.qlen + (w.q0 + n / G - s.qo) : s.len - 1, t1 - 1);
-      lim_min = min(lim_min, lim[cb]);
-    }
-  }
-#pragma unroll
-  for (int o_ = 8; o_ >= 1; o_ >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o_, 64));
-  lim_min = uniform(lim_min);
-
-  float m[NCB], lsum[NCB];
-  f32x4 o[8][NCB];
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) {
-    m[cb] = kNegInf;
-    lsum[cb] = 0.f;
-#pragma unroll
-    for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  wait_units<kBlk8Units, 5>(issued);  // Q
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-
-  for (int tok = t0 + 32 * wave; tok < t1; tok += 128) {
-    asm volatile("" : "+v"(k_at), "+v"(q_at), "+v"(v_at));  // (the derived addresses are not to be held)
-    // ---- S^T
-    wait_units<kBlk8Units, 5>(issued - consumed - 1);
-    const uint32_t kst = ring + (uint32_t)(r_slot * kKv8Slot);
-    r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
-    const f32x2 ks = *(lds_f32x2*)(uintptr_t)(kst + kKv8Unit);
-    u32x4 kw[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int tb = 0; tb < 2; ++tb) kw[i][tb] = lds_read16(kst + 2048 * tb + (k_at ^ (64 * i)));
-    u32x4 qf[2][NCB];  // this k-step's and the next one's
-    auto read_q = [&](int k) {
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb)
-        qf[k & 1][cb] = lds_read16(lbase + (q_at ^ (16 * (8 * (k >> 1) + (k & 1)))) + 4096 * cb);
-    };
-    read_q(0);
-    f32x4 sc[2][NCB];
-#pragma unroll
-    for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (k < 3) read_q(k + 1);
-      __builtin_amdgcn_sched_barrier(0);  // (else the reads sink to their use, behind a full LDS latency each)
-      u32x4 kf[2];
-#pragma unroll
-      for (int tb = 0; tb < 2; ++tb)
-        kf[tb] = kv8_decode8<BF16>(kw[k >> 1][tb][2 * (k & 1)], kw[k >> 1][tb][2 * (k & 1) + 1], ks[tb], ks[tb]);
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb) sc[tb][cb] = mfma16<BF16>(kf[tb], qf[k & 1][cb], sc[tb][cb]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  auto barrier = [&]() {  // of LDS reads and writes; copies stay in flight
     wait_lds();
-    consumed += 1;
-    refill();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  next_item();
 
-    // ---- softmax
-    if (tok + 31 > lim_min) {
+  for (int it = it0; it < it1; ++it) {
+    const WorkItem w = ldc_item(a.items, it);
+    const SeqInfo s = ldc_seq(a.seqs, w.seq);
+    const int t0 = w.t0, t1 = w.t1, kvh = w.kvh;
+    const int ncols = w.nq * G;
+
+    // Q: wavefront wv copies column block wv; columns past the item repeat its first.
+    {
+      const int before = issued;
+      const int ln = fresh_lane();
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = 4 * r + (ln >> 4);
+        const int col = 16 * wv + n;
+        const int nn = col < ncols ? col : 0;
+        lds_dma16(a.q + ((size_t)(w.q0 + nn / G) * a.hq + kvh * G + nn % G) * kHeadDim + 8 * ((ln & 15) ^ n),
+                  qbase + (uint32_t)(4096 * wv + 1024 * r));
+      }
+      refill();
+      wait_units<kBlk8Units, 5>(issued - before);
+    }
+
+    int lim[NCB];
+    int lim_min = 1 << 30;
+    const int lq = fresh_lane() & 15;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const int n = 16 * cb + lq;
+      lim[cb] = -1;
+      if (n < ncols) {
+        lim[cb] = min(CAUSAL ? s.len - s.qlen + (w.q0 + n / G - s.qo) : s.len - 1, t1 - 1);
+        lim_min = min(lim_min, lim[cb]);
+      }
+    }
+#pragma unroll
+    for (int o_ = 8; o_ >= 1; o_ >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o_, 64));
+    lim_min = uniform(lim_min);
+
+    float m[NCB], lsum[NCB];
+    f32x4 o[8][NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      m[cb] = kEmpty;
+      lsum[cb] = 0.f;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) o[db][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    barrier();  // Q is in LDS
+
+    for (int tok = t0 + 32 * wv; tok < t1; tok += 128) {
+      asm volatile("" : "+v"(k_at), "+v"(q_at), "+v"(v_at));  // (the derived addresses are not to be held)
+      // ---- S^T
+      wait_units<kBlk8Units, 5>(issued - consumed - 1);
+      const uint32_t kst = ring + (uint32_t)(r_slot * kKv8Slot);
+      r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
+      const f32x2 ks = *(lds_f32x2*)(uintptr_t)(kst + kKv8Unit);
+      u32x4 kw[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) kw[i][tb] = lds_read16(kst + 2048 * tb + (k_at ^ (64 * i)));
+      u32x4 qf[2][NCB];  // this k-step's and the next one's
+      auto read_q = [&](int k) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+          qf[k & 1][cb] = lds_read16(qbase + (q_at ^ (16 * (8 * (k >> 1) + (k & 1)))) + 4096 * cb);
+      };
+      read_q(0);
+      f32x4 sc[2][NCB];
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) sc[tb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k < 3) read_q(k + 1);
+        __builtin_amdgcn_sched_barrier(0);  // (else the reads sink to their use, behind a full LDS latency each)
+        u32x4 kf[2];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+          kf[tb] = kv8_decode8<BF16>(kw[k >> 1][tb][2 * (k & 1)], kw[k >> 1][tb][2 * (k & 1) + 1], ks[tb], ks[tb]);
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
-    }
-    // The statistics first: V^T operands are read ahead of the exponentials.
-    float alpha[NCB];
-    bool any_up = false;
+          for (int tb = 0; tb < 2; ++tb) sc[tb][cb] = mfma16<BF16>(kf[tb], qf[k & 1][cb], sc[tb][cb]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_lds();
+      consumed += 1;
+      refill();
+
+      // ---- softmax
+      if (tok + 31 > lim_min) {
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      float mx = kNegInf;
+        for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-      for (int tb = 0; tb < 2; ++tb)
+          for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[tb][cb][r]);
-      mx = max_x32(max_x16(mx));
-      const float mt = mx * a.scale_log2;
-      const bool up = mt > m[cb] + 8.f;  // lazy reference maximum, p <= 2^8
-      alpha[cb] = up ? fast_exp2(m[cb] - mt) : 1.f;
-      if (up) m[cb] = mt;
-      any_up = any_up || up;
-    }
-    if (__builtin_amdgcn_ballot_w64(any_up) != 0) {
+            for (int r = 0; r < 4; ++r)
+              if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
+      }
+      // The statistics first: V^T operands are read ahead of the exponentials.
+      float mx[NCB];
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
-        lsum[cb] *= alpha[cb];
+        mx[cb] = kNegInf;
 #pragma unroll
-        for (int db = 0; db < 8; ++db) o[db][cb] *= alpha[cb];
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
       }
-    }
-    wait_units<kBlk8Units, 5>(issued - consumed - 1);
-    const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
-    r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
-    if (t1 - tok < 32) {
-      // rows past the item end: zero (0 * stale must stay 0)
+      raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
+      wait_units<kBlk8Units, 5>(issued - consumed - 1);
+      const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
+      r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
+      if (t1 - tok < 32) {
+        // rows past the item end: zero (0 * stale must stay 0)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int q = lane + 64 * u;
-        if ((q >> 3) >= t1 - tok) lds_zero16(vst + 16 * q);
+        for (int u = 0; u < 4; ++u) {
+          const int q = lane + 64 * u;
+          if ((q >> 3) >= t1 - tok) lds_zero16(vst + 16 * q);
+        }
       }
-    }
-    const f32x2 vs = *(lds_f32x2*)(uintptr_t)(vst + kKv8Unit);
-    u32x2 vw[8];
+      const f32x2 vs = *(lds_f32x2*)(uintptr_t)(vst + kKv8Unit);
+      u32x2 vw[8];
 #pragma unroll
-    for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + (v_at ^ (16 * db)));
-    __builtin_amdgcn_sched_barrier(0);
-    u32x4 pf[NCB];
+      for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + (v_at ^ (16 * db)));
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 pf[NCB];
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        float x[2][4];
+        float ps = 0.f;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
+            ps += x[tb][r];
+          }
+        lsum[cb] += ps;
+        pf[cb] = u32x4{pack2<BF16>(x[0][0], x[0][1]), pack2<BF16>(x[0][2], x[0][3]), pack2<BF16>(x[1][0], x[1][1]),
+                       pack2<BF16>(x[1][2], x[1][3])};
+      }
+
+      // ---- O^T
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        const u32x4 vf = kv8_decode8<BF16>(vw[db][0], vw[db][1], vs[0], vs[1]);
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[cb], o[db][cb]);
+      }
+      wait_lds();
+      consumed += 1;
+      refill();
+    }
+
+    // ---- combine, 16 columns a round: wavefront v finishes dims 32 v .. + 31,
+    // which the other three hand it.
+    const int ln = fresh_lane(), Jc = ln >> 4, Lc = ln & 15;
+    const uint32_t stats = qbase + kBlk8Stats;
+    barrier();  // every step's reads of Q are done
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      const float m_use = m[cb] == kNegInf ? 0.f : m[cb];
-      float x[2][4];
-      float ps = 0.f;
+      lsum[cb] = sum_x32(sum_x16(lsum[cb]));
+      float mx = 0.f;
 #pragma unroll
-      for (int tb = 0; tb < 2; ++tb)
+      for (int db = 0; db < 8; ++db)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m_use));
-          ps += x[tb][r];
-        }
-      lsum[cb] += ps;
-      pf[cb] = u32x4{pack2<BF16>(x[0][0], x[0][1]), pack2<BF16>(x[0][2], x[0][3]), pack2<BF16>(x[1][0], x[1][1]),
-                     pack2<BF16>(x[1][2], x[1][3])};
-    }
-
-    // ---- O^T
-#pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      const u32x4 vf = kv8_decode8<BF16>(vw[db][0], vw[db][1], vs[0], vs[1]);
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pf[cb], o[db][cb]);
-    }
-    wait_lds();
-    consumed += 1;
-    refill();
-  }
-
-  // ---- combine, 32 columns a round: row = column, 16-byte chunk c (dims 4 c
-  // ..) at chunk position c ^ (column % 16)
-  const uint32_t mine = lbase + (uint32_t)(16384 * wave);
-  const uint32_t stats = lbase + kBlk8Stats;
-  const int c = lane & 31;
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) lsum[cb] = sum_x32(sum_x16(lsum[cb]));
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    if (32 * half < ncols) {
-      __syncthreads();  // the steps' (the other half's) reads are done
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int cb = 2 * half + i;
-#pragma unroll
-        for (int db = 0; db < 8; ++db)
-          *(lds_f32x4*)(uintptr_t)(mine + (uint32_t)(512 * (16 * i + L) + 16 * ((4 * db + J) ^ L))) = o[db][cb];
-        if (J == 0) {
-          const f32x2 st = {m[cb], lsum[cb]};
-          *(lds_f32x2*)(uintptr_t)(stats + (uint32_t)(8 * (64 * wave + 16 * cb + L))) = st;
-        }
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, fabsf(o[db][cb][r]));
+      mx = max_x32(max_x16(mx));
+      if (Jc == 0) {
+        const uint32_t at = stats + (uint32_t)(12 * (64 * wv + 16 * cb + Lc));
+        *(lds_f32*)(uintptr_t)at = m[cb];
+        *(lds_f32*)(uintptr_t)(at + 4) = lsum[cb];
+        *(lds_f32*)(uintptr_t)(at + 8) = mx;
       }
-      __syncthreads();
-      for (int n = 2 * wave + (lane >> 5); n < 32; n += 8) {
-        const int col = 32 * half + n;
-        if (col >= ncols) break;
-        f32x2 st[4];
+    }
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      if (16 * cb < ncols) {
+        if (cb > 0) barrier();  // the round before is read
+        f32x4 acc[2];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          if (v == wv) {
+            acc[0] = o[2 * v][cb];
+            acc[1] = o[2 * v + 1][cb];
+          } else {
+            const uint32_t to = qbase + (uint32_t)(2048 * (3 * v + (wv < v ? wv : wv - 1)) + 16 * ln);
+            *(lds_f32x4*)(uintptr_t)to = o[2 * v][cb];
+            *(lds_f32x4*)(uintptr_t)(to + 1024) = o[2 * v + 1][cb];
+          }
+        }
+        barrier();
+        float mv[4], lv[4], xv[4];
         float top = kNegInf;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          st[v] = *(lds_f32x2*)(uintptr_t)(stats + (uint32_t)(8 * (64 * v + col)));
-          top = fmaxf(top, st[v][0]);
+          const uint32_t at = stats + (uint32_t)(12 * (64 * v + 16 * cb + Lc));
+          mv[v] = *(lds_f32*)(uintptr_t)at;
+          lv[v] = *(lds_f32*)(uintptr_t)(at + 4);
+          xv[v] = *(lds_f32*)(uintptr_t)(at + 8);
+          top = fmaxf(top, mv[v]);
         }
-        const float base = top == kNegInf ? 0.f : top;
-        float ls = 0.f;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        const float base = top;
+        float ls = 0.f, bound = 0.f, own = 0.f;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float wt = fast_exp2(st[v][0] - base);
-          ls += st[v][1] * wt;
-          acc += *(lds_f32x4*)(uintptr_t)(lbase + (uint32_t)(16384 * v + 512 * n + 16 * (c ^ (n & 15)))) * wt;
+          mv[v] = fast_exp2(mv[v] - base);
+          ls += lv[v] * mv[v];
+          bound += xv[v] * mv[v];
+          if (v == wv) own = mv[v];
         }
-        const int r = col / G, head = kvh * G + (col - r * G);
-        put_combined<BF16>(a, acc, ls, top, w.part, w.q0 + r, w.part + r, head, c);
+        acc[0] *= own;
+        acc[1] *= own;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          if (v == wv) continue;
+          const uint32_t from = qbase + (uint32_t)(2048 * (3 * wv + (v < wv ? v : v - 1)) + 16 * ln);
+          acc[0] += *(lds_f32x4*)(uintptr_t)from * mv[v];
+          acc[1] += *(lds_f32x4*)(uintptr_t)(from + 1024) * mv[v];
+        }
+        const int col = 16 * cb + Lc;
+        if (col < ncols) {
+          const float inv = ls > 0.f ? 1.f / ls : 0.f;
+          const float l2 = ls > 0.f ? top + __log2f(ls) : kNegInf;
+          const int r = col / G, head = kvh * G + (col - r * G);
+          acc[0] *= inv;
+          acc[1] *= inv;
+          if (w.part < 0) {
+            const size_t oi = (size_t)(w.q0 + r) * a.hq + head;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<u32x2*>(a.out + oi * kHeadDim + 32 * wv + 16 * i + 4 * Jc) =
+                  u32x2{pack2<BF16>(acc[i][0], acc[i][1]), pack2<BF16>(acc[i][2], acc[i][3])};
+            if (a.lse != nullptr && wv == 0 && Jc == 0) a.lse[oi] = l2 * kLn2;
+          } else {
+            // (the parts' largest magnitudes bound the row's: within a few times)
+            float is;
+            const float sc = part_scale_of(bound * inv, is);
+            const size_t oi = (size_t)(w.part + r) * a.hq + head;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<u32x2*>(a.part_o + oi * kHeadDim + 32 * wv + 16 * i + 4 * Jc) =
+                  u32x2{pack2<false>(acc[i][0] * is, acc[i][1] * is), pack2<false>(acc[i][2] * is, acc[i][3] * is)};
+            if (wv == 0 && Jc == 0) {
+              a.part_lse[oi] = l2;
+              a.part_scale[oi] = sc;
+            }
+          }
+        }
       }
     }
+    if (it + 1 < it1) barrier();  // the region is the next item's Q
   }
 }
 
-// Narrow: every item has at most 64 columns.  Wide: any items, as tiles.  Any:
-// the launch of a graph plan, whose later prepares may bring either kind.
-// (One kernel with all paths for the eager launches too takes 262 us for 8192
-// prompt tokens, 234 without the narrow items' path beside it.)
-enum class Tile8 { Narrow, Wide, Any };
+template <bool BF16, bool CAUSAL, bool STREAM, int HEADS>
+__global__ __launch_bounds__(256 * HEADS, 2) void attn_block_kv8_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t dsm[];
+  const int wave = uniform(threadIdx.x >> 6);
+  const uint32_t lbase = (uint32_t)(uintptr_t)dsm;
+  // Workgroups of one XCD (every eighth) take neighbouring shares, the kv heads
+  // of one token range, so that its L2 channels see all of a page's lines.
+  const int n_wg = (int)gridDim.x;
+  const int b = n_wg % 8 == 0 ? (int)(blockIdx.x % 8) * (n_wg / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+  const int share = HEADS * b + (wave >> 2);
+  const int it = ldc(a.tile_off, share);
+  const int end = min(ldc(a.tile_off, share + 1), uniform(*a.n_items));
+  if (it >= end) return;
+  block8_items<BF16, CAUSAL, STREAM>(a, it, end, lbase + (uint32_t)((wave >> 2) * kBlk8Head),
+                                     lbase + (uint32_t)(HEADS * kBlk8Head + wave * kBlk8Wave), wave & 3,
+                                     threadIdx.x & 63);
+}
+
+// Wide: any items, as tiles.  Any: the launch of a graph plan, whose later
+// prepares may bring either kind: items of at most 64 columns as blocks.  (That
+// one for eager launches too takes 262 us for 8192 prompt tokens, 234 without
+// the narrow items' path beside it.)
+enum class Tile8 { Wide, Any };
 
 template <bool BF16, bool CAUSAL, bool STREAM, Tile8 KIND>
 __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
@@ -1325,15 +1414,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
   Tile8Lanes tl;
   if constexpr (KIND == Tile8::Wide) tl = tile8_lanes(a, lane);
 
-  // Narrow: workgroups of one XCD (every eighth) take neighbouring shares, the
-  // kv heads of one token range where the list is an equal cut, so that an
-  // XCD's L2 channels see all of a page's lines instead of one head's (32
-  // draft blocks over 2048..16384 tokens: 147 us a call, 156 in plain order).
-  const int n_wg = (int)gridDim.x;
-  const int b = KIND == Tile8::Narrow && n_wg % 8 == 0 ? (int)(blockIdx.x % 8) * (n_wg / 8) + (int)blockIdx.x / 8
-                                                        : (int)blockIdx.x;
-  int it = ldc(a.tile_off, b);
-  const int end = min(ldc(a.tile_off, b + 1), n_items);
+  int it = ldc(a.tile_off, blockIdx.x);
+  const int end = min(ldc(a.tile_off, blockIdx.x + 1), n_items);
   if (it >= end) return;
   WorkItem w = ldc_item(a.items, it);
   SeqInfo s = ldc_seq(a.seqs, w.seq);
@@ -1356,9 +1438,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
         stage = tile8_item<BF16, CAUSAL, 1, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
       else
         stage = tile8_item<BF16, CAUSAL, 2, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
-    } else if (KIND == Tile8::Narrow || w.nq * a.group <= 64) {
-      block8_item<BF16, CAUSAL, STREAM>(a, w, s, lbase, wave, fresh_lane());
-    } else if constexpr (KIND == Tile8::Any) {
+    } else if (w.nq * a.group <= 64) {
+      block8_items<BF16, CAUSAL, STREAM>(a, it, it + 1, lbase, lbase + (uint32_t)(kBlk8Head + wave * kBlk8Wave), wave,
+                                         fresh_lane());
+    } else {
       const int ln = fresh_lane();
       const Tile8Lanes tw = tile8_lanes(a, ln);
       if (!primed) scales = tile8_copy<STREAM>(a, w, s, tw.goff, lbase, wave, w.t0);
@@ -1441,25 +1524,40 @@ static hipError_t tile8_launch(const AttnArgs& a, int grid, hipStream_t st) {
   return hipGetLastError();
 }
 
+// (HEADS = 2: `grid` shares are an equal cut's, all kv heads of a token range
+// together, so that neighbours have the same items.)
+template <bool BF16, bool CAUSAL, bool STREAM, int HEADS>
+static hipError_t block8_launch(const AttnArgs& a, int grid, hipStream_t st) {
+  constexpr size_t lds = (size_t)HEADS * kTile8Lds;
+  static std::atomic<uint64_t> lds_ok{0};
+  const hipError_t e = allow_lds((const void*)attn_block_kv8_kernel<BF16, CAUSAL, STREAM, HEADS>, lds, lds_ok);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((attn_block_kv8_kernel<BF16, CAUSAL, STREAM, HEADS>), dim3(grid / HEADS), dim3(256 * HEADS), lds,
+                     st, a);
+  return hipGetLastError();
+}
+
 template <bool BF16, bool CAUSAL>
-static hipError_t tile8_kind(const AttnArgs& a, bool stream, bool any, bool narrow, int grid, hipStream_t st) {
+static hipError_t tile8_kind(const AttnArgs& a, bool stream, bool any, bool narrow, bool pairs, int grid,
+                             hipStream_t st) {
   auto go = [&](auto streamed) {
     constexpr bool S = decltype(streamed)::value;
     if (any) return tile8_launch<BF16, CAUSAL, S, Tile8::Any>(a, grid, st);
-    return narrow ? tile8_launch<BF16, CAUSAL, S, Tile8::Narrow>(a, grid, st)
-                  : tile8_launch<BF16, CAUSAL, S, Tile8::Wide>(a, grid, st);
+    if (!narrow) return tile8_launch<BF16, CAUSAL, S, Tile8::Wide>(a, grid, st);
+    return pairs ? block8_launch<BF16, CAUSAL, S, 2>(a, grid, st) : block8_launch<BF16, CAUSAL, S, 1>(a, grid, st);
   };
   return stream ? go(std::true_type{}) : go(std::false_type{});
 }
 
-// any: a graph plan's launch; else narrow: every item has at most 64 columns.
-hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, bool any, bool narrow, int grid,
-                           hipStream_t st) {
+// any: a graph plan's launch; else narrow: every item has at most 64 columns;
+// pairs: and the list is an equal cut over an even number of kv heads.
+hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, bool any, bool narrow, bool pairs,
+                           int grid, hipStream_t st) {
   if (bf16)
-    return causal ? tile8_kind<true, true>(a, stream, any, narrow, grid, st)
-                  : tile8_kind<true, false>(a, stream, any, narrow, grid, st);
-  return causal ? tile8_kind<false, true>(a, stream, any, narrow, grid, st)
-                : tile8_kind<false, false>(a, stream, any, narrow, grid, st);
+    return causal ? tile8_kind<true, true>(a, stream, any, narrow, pairs, grid, st)
+                  : tile8_kind<true, false>(a, stream, any, narrow, pairs, grid, st);
+  return causal ? tile8_kind<false, true>(a, stream, any, narrow, pairs, grid, st)
+                : tile8_kind<false, false>(a, stream, any, narrow, pairs, grid, st);
 }
 
 }  // namespace feattn

@@ -31,8 +31,8 @@ int decode_wg_waves(int hkv);
 hipError_t launch_tile(const AttnArgs& a, bool bf16, bool causal, bool stream, int grid, hipStream_t st);
 hipError_t launch_decode_kv8(const AttnArgs& a, bool bf16, int waves, int ncb, int causal, bool any, int grid,
                              hipStream_t st);
-hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, bool any, bool narrow, int grid,
-                           hipStream_t st);
+hipError_t launch_tile_kv8(const AttnArgs& a, bool bf16, bool causal, bool stream, bool any, bool narrow, bool pairs,
+                           int grid, hipStream_t st);
 hipError_t launch_merge(const MergeArgs& a, bool bf16, int grid, hipStream_t st);
 hipError_t launch_stage_copy(void* dst, const void* src, size_t bytes, hipStream_t st);
 hipError_t launch_rope(void* q, void* k, const int64_t* pos, const float* cache, int rows, int hq, int hkv, int dim,
@@ -332,6 +332,7 @@ struct Launch {
   int graph_tile = -1;  // graph plans: the first graph prepare had tile work (1) or not (0)
   bool tile_stream[2] = {true, true};  // tile K/V reads with the non-temporal hint, per mask mode
   bool tile_narrow[2] = {false, false};  // no tile item of more than 64 columns
+  bool tile_cut[2] = {false, false};     // the tile list is an equal cut (cut_tile_stream)
   int graph_stream[2] = {-1, -1};      // graph plans: that choice at the first graph prepare
   int n_decode = 0, n_tile[2] = {0, 0}, n_merge[2] = {0, 0};
   int n_pieces = 0, tile_rows[2] = {0, 0};  // reported only
@@ -388,6 +389,7 @@ void record_lists(Launch& L, const BuiltPlan& bp, const HeapPlace& hp, int nc) {
     L.n_tile[m] = (int)bp.mode[m].tile.size();
     L.tile_rows[m] = bp.mode[m].tile.empty() ? 0 : bp.mode[m].tile_rows;
     L.n_tshare[m] = bp.mode[m].tile_off.empty() ? 0 : (int)bp.mode[m].tile_off.size() - 1;
+    L.tile_cut[m] = bp.mode[m].cut;
     L.tile_narrow[m] = true;
     for (const SeqInfo& s : bp.seqs)
       if (std::min(s.qlen, bp.mode[m].tile_rows) * (L.sh.hq / L.sh.hkv) > 64) L.tile_narrow[m] = false;
@@ -527,7 +529,8 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
     t.tile_off = reinterpret_cast<const int32_t*>(L.dev + L.lay.tshare[mode]);
     const int grid = L.graph ? L.grid_tile_cap : L.n_tshare[mode];
     e = scales != nullptr ? launch_tile_kv8(t, L.bf16, causal != 0, L.tile_stream[mode], L.graph,
-                                            L.tile_narrow[mode], std::max(grid, 1), st)
+                                            L.tile_narrow[mode], L.tile_cut[mode] && L.sh.hkv % 2 == 0,
+                                            std::max(grid, 1), st)
                           : launch_tile(t, L.bf16, causal != 0, L.tile_stream[mode], std::max(grid, 1), st);
     if (e != hipSuccess) return hip_fail(e, "tile kernel launch");
   }

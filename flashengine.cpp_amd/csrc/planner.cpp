@@ -170,6 +170,7 @@ bool cut_tile_stream(const std::vector<SeqInfo>& seqs, int G, int hkv, bool caus
   if (rows > slot_budget) return false;
 
   ModeLists out;
+  out.cut = true;
   out.tile_rows = qr;
   out.partial_rows = (int)rows;
   for (size_t i = 0; i < ch.size(); ++i)

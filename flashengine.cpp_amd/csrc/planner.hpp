@@ -30,6 +30,7 @@ struct ModeLists {
   std::vector<WorkItem> tile;            // grouped by share: share k = [tile_off[k], tile_off[k+1])
   std::vector<int32_t> tile_off;         // CSR over shares (one share per tile workgroup)
   int tile_rows = 0;                     // query rows of a tile item at most
+  bool cut = false;                      // an equal cut: shares k hkv .. + hkv - 1 are the kv heads of the same pieces
   std::vector<MergeRow> merge;
   int partial_rows = 0;  // decode partials followed by this mode's tile partials
 };
