@@ -35,29 +35,59 @@ __device__ __forceinline__ int swz_v(int t) {
 // with it need no special case.)
 constexpr float kEmpty = -3.4028234663852886e38f;
 
-// The running reference maximum m of each column, in log2 units, is lazy: it is
-// raised, and l and o with it rescaled, only where a step's maximum exceeds it
-// by more than 8, so that p <= 2^8.  Whether any does needs no exchange between
-// the lanes of a column: each compares its own maximum mx, and the vote of the
-// wavefront stands for the rest.  (With the columns' maxima exchanged every step,
-// draft blocks took @BLOCKS@, prefill @PREFILL@.)
-template <int NCB>
-__device__ __forceinline__ void raise_max(const float (&mx)[NCB], float scale, float (&m)[NCB], float (&lsum)[NCB],
-                                          f32x4 (&o)[8][NCB]) {
+// Softmax of a step's scores against the running reference maximum m of each
+// column, in log2 units, which is lazy: the probabilities p = 2^(s scale - m) are
+// taken with the m there is, and only where a lane's sum of them passes 2^9 (so
+// that a single one might, or is infinite: a column's first step) is m raised to
+// the column's maximum, l and o with it rescaled, and the step taken again.  No
+// maximum and no exchange between the lanes of a column otherwise.  (With the
+// columns' maxima exchanged every step 32 draft blocks took 147 us and 2048 rows
+// over 30000 1105 us, with each lane's maximum compared 143 and 1070.)
+// P: the step's 16-token blocks; put(cb, p) takes a column block's values.
+template <int P, int NCB, typename PUT>
+__device__ __forceinline__ void softmax_step(f32x4 (&sc)[P][NCB], float scale, float (&m)[NCB], float (&lsum)[NCB],
+                                             f32x4 (&o)[8][NCB], PUT put) {
+  constexpr float kMost = 512.f;
+  float ps[NCB];
+  auto exponentials = [&](int cb) {
+    float x[P][4];
+    float t = 0.f;
+#pragma unroll
+    for (int tb = 0; tb < P; ++tb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], scale, -m[cb]));
+        t += x[tb][r];
+      }
+    ps[cb] = t;
+    put(cb, x);
+  };
   bool above = false;
 #pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) above = above || mx[cb] * scale > m[cb] + 8.f;
-  if (__builtin_amdgcn_ballot_w64(above) == 0) return;
-#pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
-    const float mt = max_x32(max_x16(mx[cb])) * scale;
-    const bool up = mt > m[cb] + 8.f;
-    const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
-    if (up) m[cb] = mt;
-    lsum[cb] *= alpha;
-#pragma unroll
-    for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
+    exponentials(cb);
+    above = above || ps[cb] > kMost;
   }
+  if (__builtin_amdgcn_ballot_w64(above) != 0) {
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int tb = 0; tb < P; ++tb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[tb][cb][r]);
+      const float mt = max_x32(max_x16(mx)) * scale;
+      const bool up = mt > m[cb];
+      const float alpha = up ? fast_exp2(m[cb] - mt) : 1.f;
+      if (up) m[cb] = mt;
+      lsum[cb] *= alpha;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) o[db][cb] *= alpha;
+      exponentials(cb);
+    }
+  }
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) lsum[cb] += ps[cb];
 }
 
 // Probabilities as two 16-bit operands whose sum they are within 2^-17 (bf16) or
@@ -333,35 +363,18 @@ __device__ __forceinline__ void short_items_kv8(const AttnArgs& a, int causal, i
           load_k();  // under the softmax
         }
 
-        float mx[NCB];
 #pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-          mx[cb] = kNegInf;
+        for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
           for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < 4; ++r)
               if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
-              mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
-            }
-        }
-        raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
         u32x4 pf[2][NCB], pl[2][NCB];
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-          float x[4][4];
-          float ps = 0.f;
-#pragma unroll
-          for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
-              ps += x[tb][r];
-            }
-          lsum[cb] += ps;
+        softmax_step<4, NCB>(sc, a.scale_log2, m, lsum, o, [&](int cb, const float (&x)[4][4]) {
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) pack8_split<BF16>(x[2 * ks], x[2 * ks + 1], pf[ks][cb], pl[ks][cb]);
-        }
+        });
 
         __builtin_amdgcn_sched_barrier(0);
         // V rows past the last token, up to the 32-token step they end in,
@@ -685,21 +698,15 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
         }
       }
 
-      // ---- softmax: the statistics, then the exponentials under the reads of V
-      float mx[NCB];
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        mx[cb] = kNegInf;
+      for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
+          for (int r = 0; r < 4; ++r)
             if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
-            mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
-          }
-      }
-      raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
 
+      // ---- the reads of V, and the exponentials under them
       wait_units<U, 5>(issued - consumed - 1);
       const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
       r_slot = r_slot + 1 == U ? 0 : r_slot + 1;
@@ -718,20 +725,9 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
       for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + v_lds[db]);
       __builtin_amdgcn_sched_barrier(0);
       u32x4 pf[NCB], pl[NCB];
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        float x[2][4];
-        float ps = 0.f;
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
-            ps += x[tb][r];
-          }
-        lsum[cb] += ps;
+      softmax_step<2, NCB>(sc, a.scale_log2, m, lsum, o, [&](int cb, const float (&x)[2][4]) {
         pack8_split<BF16>(x[0], x[1], pf[cb], pl[cb]);
-      }
+      });
 
       // ---- O^T
 #pragma unroll
@@ -764,8 +760,8 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
 // Four wavefronts share 64-token tiles.  Wavefront w copies the codes of block
 // w of the next tile to a region of its own (4 KB) while the current one is
 // computed; once they have landed it converts them, once for all four, into
-// the 16-bit tile (32 KB: K blocks, then V blocks, 16 tokens x 256 bytes; chunk
-// c of row t at c ^ t in K, c ^ 2t in V), of which there are two.
+// the 16-bit tile (32 KB: K blocks, then V blocks, 16 tokens x 256 bytes, the
+// chunks of a row permuted), of which there are two.
 constexpr int kTile8Block = 4096;
 constexpr int kTile8Stage = 8 * kTile8Block;
 constexpr int kTile8Raw = 2 * kTile8Stage;           // offset of the wavefronts' code regions
@@ -784,19 +780,28 @@ struct Tile8Lanes {
   uint32_t k_lds[4], v_lds[8];
 };
 
+// Row of a block that a lane copies and converts in instruction u, and the
+// chunk positions (c ^ these) of row t in the 16-bit tile: rows t and t + 8, of
+// neighbouring groups of eight lanes, differ in the lowest bit, so that the
+// lanes' even (and odd) chunks of both meet no bank twice; the operand reads,
+// of 16 rows (K) and of eight consecutive ones (V), do not either.
+__device__ __forceinline__ int tile8_row(int lane, int u) { return 8 * ((lane >> 3) & 1) + (lane >> 4) + 4 * u; }
+__device__ __forceinline__ int tile8_swz_k(int t) { return t ^ (t >> 3); }
+__device__ __forceinline__ int tile8_swz_v(int t) { return ((2 * t) & 15) | (t >> 3); }
+
 __device__ __forceinline__ Tile8Lanes tile8_lanes(const AttnArgs& a, int lane) {
   const int J = lane >> 4, L = lane & 15;
   const int row_bytes = a.hkv * kHeadDim;
   Tile8Lanes tl;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)((8 * r + (lane >> 3)) * row_bytes + 16 * (lane & 7));
+  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)(tile8_row(lane, r) * row_bytes + 16 * (lane & 7));
 #pragma unroll
-  for (int s = 0; s < 4; ++s) tl.k_lds[s] = (uint32_t)(16 * (16 * L + (((4 * s + J) ^ L) & 15)));
+  for (int s = 0; s < 4; ++s) tl.k_lds[s] = (uint32_t)(16 * (16 * L + ((4 * s + J) ^ tile8_swz_k(L))));
   const int k = L >> 2, m = L & 3, t = 4 * J + k;
 #pragma unroll
   for (int db = 0; db < 8; ++db) {
     const int c = 2 * db + (m >> 1);
-    tl.v_lds[db] = (uint32_t)(16 * (16 * t + ((c ^ (2 * t)) & 15)) + 8 * (m & 1));
+    tl.v_lds[db] = (uint32_t)(16 * (16 * t + (c ^ tile8_swz_v(t))) + 8 * (m & 1));
   }
   return tl;
 }
@@ -891,40 +896,23 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
       }
     }
 
-    float mx[NCB];
+    if constexpr (MASK) {
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      mx[cb] = kNegInf;
+      for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-      for (int tb = 0; tb < 4; ++tb)
+        for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (MASK) {
+          for (int r = 0; r < 4; ++r)
             if (T + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
-          }
-          mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
-        }
     }
-    raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
     u32x4 pf[2][NCB];
-#pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      float x[4][4];
-      float ps = 0.f;
-#pragma unroll
-      for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
-          ps += x[tb][r];
-        }
-      lsum[cb] += ps;
+    softmax_step<4, NCB>(sc, a.scale_log2, m, lsum, o, [&](int cb, const float (&x)[4][4]) {
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
         pf[ks][cb] = u32x4{pack2<BF16>(x[2 * ks][0], x[2 * ks][1]), pack2<BF16>(x[2 * ks][2], x[2 * ks][3]),
                            pack2<BF16>(x[2 * ks + 1][0], x[2 * ks + 1][1]),
                            pack2<BF16>(x[2 * ks + 1][2], x[2 * ks + 1][3])};
-    }
+    });
 
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
@@ -958,7 +946,7 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
       const int c = lane & 7;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int t = 8 * u + (lane >> 3);
+        const int t = tile8_row(lane, u);
         const u32x4 kw = lds_read16(raw + 16 * lane + 1024 * u);
         u32x4 vw = lds_read16(raw + 2048 + 16 * lane + 1024 * u);
         if (t >= valid) vw = u32x4{0u, 0u, 0u, 0u};
@@ -966,9 +954,9 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
         const uint32_t vd = kd + 4 * kTile8Block;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          lds_write16(kd + 16 * (((2 * c + h) ^ t) & 15),
+          lds_write16(kd + 16 * ((2 * c + h) ^ tile8_swz_k(t)),
                       kv8_decode8<BF16>(kw[2 * h], kw[2 * h + 1], scales[0], scales[0]));
-          lds_write16(vd + 16 * (((2 * c + h) ^ (2 * t)) & 15),
+          lds_write16(vd + 16 * ((2 * c + h) ^ tile8_swz_v(t)),
                       kv8_decode8<BF16>(vw[2 * h], vw[2 * h + 1], scales[1], scales[1]));
         }
       }
@@ -1221,17 +1209,7 @@ __device__ __forceinline__ void block8_items(const AttnArgs& a, int it0, int it1
             for (int r = 0; r < 4; ++r)
               if (tok + 16 * tb + 4 * J + r > lim[cb]) sc[tb][cb][r] = kNegInf;
       }
-      // The statistics first: V^T operands are read ahead of the exponentials.
-      float mx[NCB];
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        mx[cb] = kNegInf;
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) mx[cb] = fmaxf(mx[cb], sc[tb][cb][r]);
-      }
-      raise_max<NCB>(mx, a.scale_log2, m, lsum, o);
+      // (V^T operands are read ahead of the exponentials)
       wait_units<kBlk8Units, 5>(issued - consumed - 1);
       const uint32_t vst = ring + (uint32_t)(r_slot * kKv8Slot);
       r_slot = r_slot + 1 == kBlk8Units ? 0 : r_slot + 1;
@@ -1249,21 +1227,10 @@ __device__ __forceinline__ void block8_items(const AttnArgs& a, int it0, int it1
       for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + (v_at ^ (16 * db)));
       __builtin_amdgcn_sched_barrier(0);
       u32x4 pf[NCB];
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        float x[2][4];
-        float ps = 0.f;
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[tb][r] = fast_exp2(__builtin_fmaf(sc[tb][cb][r], a.scale_log2, -m[cb]));
-            ps += x[tb][r];
-          }
-        lsum[cb] += ps;
+      softmax_step<2, NCB>(sc, a.scale_log2, m, lsum, o, [&](int cb, const float (&x)[2][4]) {
         pf[cb] = u32x4{pack2<BF16>(x[0][0], x[0][1]), pack2<BF16>(x[0][2], x[0][3]), pack2<BF16>(x[1][0], x[1][1]),
                        pack2<BF16>(x[1][2], x[1][3])};
-      }
+      });
 
       // ---- O^T
 #pragma unroll
