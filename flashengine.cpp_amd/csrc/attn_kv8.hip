@@ -1369,11 +1369,48 @@ __global__ __launch_bounds__(256 * HEADS, 2) void attn_block_kv8_kernel(AttnArgs
                                      threadIdx.x & 63);
 }
 
-// Wide: any items, as tiles.  Any: the launch of a graph plan, whose later
+// Wide: any items, as tiles.  Even: the same, with the two shares of a compute
+// unit evened out.  Any: the launch of a graph plan, whose later
 // prepares may bring either kind: items of at most 64 columns as blocks.  (That
-// one for eager launches too takes 262 us for 8192 prompt tokens, 234 without
+// one for eager launches too took 262 us for 8192 prompt tokens, 234 without
 // the narrow items' path beside it.)
-enum class Tile8 { Wide, Any };
+enum class Tile8 { Wide, Even, Any };
+
+// The planner's longest-first lists give the first-dispatched workgroup of a
+// compute unit's two (share b < pair) 3/2 of the other's work, what the 16-bit
+// kernel's unequal pairs get through in the same time.  Here a wavefront's
+// priority at the copies keeps the two alike: the last items of share b, from
+// the one whose middle lies past half of both shares, go to share b + pair
+// (8192 prompt tokens 219 us, 234 as listed, 221 at 5/9).  Both workgroups read
+// the costs and come to the same border; who takes an item changes no result.
+__device__ __forceinline__ void tile8_even_out(const AttnArgs& a, int n_items, int lane, int& last, int& more,
+                                               int& more_end) {
+  const int b = (int)blockIdx.x;
+  const int first = b < a.pair ? b : b - a.pair;
+  const int second = first + a.pair;
+  if (second >= (int)gridDim.x) return;
+  const int a0 = ldc(a.tile_off, first), a1 = min(ldc(a.tile_off, first + 1), n_items);
+  const int b0 = ldc(a.tile_off, second), b1 = min(ldc(a.tile_off, second + 1), n_items);
+  if (a0 >= a1 || b0 >= b1) return;          // an empty share's workgroup has ended
+  if (a1 - a0 > 64 || b1 - b0 > 64) return;  // more than a lane each: left as listed
+  const int ca = lane < a1 - a0 ? a.items[a0 + lane].cost : 0;
+  int both = ca + (lane < b1 - b0 ? a.items[b0 + lane].cost : 0);
+  int upto = ca;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += v;
+    both += __shfl_xor(both, d, 64);
+  }
+  const bool keeps = lane < a1 - a0 && 2 * upto - ca <= both;
+  const int border = a0 + (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(keeps));
+  if (b == first) {
+    last = max(border, a0 + 1);
+  } else {
+    more = max(border, a0 + 1);
+    more_end = a1;
+  }
+}
 
 template <bool BF16, bool CAUSAL, bool STREAM, Tile8 KIND>
 __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
@@ -1385,7 +1422,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
   const uint32_t lbase = (uint32_t)(uintptr_t)dsm;
 
   Tile8Lanes tl;
-  if constexpr (KIND == Tile8::Wide) tl = tile8_lanes(a, lane);
+  if constexpr (KIND != Tile8::Any) tl = tile8_lanes(a, lane);
 
   int it = ldc(a.tile_off, blockIdx.x);
   const int end = min(ldc(a.tile_off, blockIdx.x + 1), n_items);
@@ -1395,18 +1432,26 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kv8_kernel(AttnArgs a) {
   f32x2 scales = {1.f, 1.f};
   int stage = 0;
   bool primed = false;  // w's first tile was requested during the item before
+  int last = end, more = 0, more_end = 0;  // this workgroup's items: [it, last), then [more, more_end)
+  if constexpr (KIND != Tile8::Any) {
+    scales = tile8_copy<STREAM>(a, w, s, tl.goff, lbase, wave, w.t0);
+    primed = true;
+  }
+  if constexpr (KIND == Tile8::Even) tile8_even_out(a, n_items, lane, last, more, more_end);
   for (;;) {
-    const int nit = it + 1;
-    const bool has_next = nit < end;
+    int nit = it + 1;
+    bool has_next = nit < end;
+    if constexpr (KIND == Tile8::Even) {
+      if (nit == last) nit = more;
+      has_next = nit != more_end && (nit < last || more < more_end);
+    }
     WorkItem wn = w;
     SeqInfo sn = s;
     if (has_next) {
       wn = ldc_item(a.items, nit);
       sn = ldc_seq(a.seqs, wn.seq);
     }
-    if constexpr (KIND == Tile8::Wide) {
-      if (!primed) scales = tile8_copy<STREAM>(a, w, s, tl.goff, lbase, wave, w.t0);
-      primed = has_next;
+    if constexpr (KIND != Tile8::Any) {
       if (w.nq * a.group <= 64)
         stage = tile8_item<BF16, CAUSAL, 1, STREAM>(a, w, s, has_next, wn, sn, tl, lbase, wave, lane, stage, scales);
       else
@@ -1516,7 +1561,9 @@ static hipError_t tile8_kind(const AttnArgs& a, bool stream, bool any, bool narr
   auto go = [&](auto streamed) {
     constexpr bool S = decltype(streamed)::value;
     if (any) return tile8_launch<BF16, CAUSAL, S, Tile8::Any>(a, grid, st);
-    if (!narrow) return tile8_launch<BF16, CAUSAL, S, Tile8::Wide>(a, grid, st);
+    if (!narrow)
+      return a.pair > 0 ? tile8_launch<BF16, CAUSAL, S, Tile8::Even>(a, grid, st)
+                        : tile8_launch<BF16, CAUSAL, S, Tile8::Wide>(a, grid, st);
     return pairs ? block8_launch<BF16, CAUSAL, S, 2>(a, grid, st) : block8_launch<BF16, CAUSAL, S, 1>(a, grid, st);
   };
   return stream ? go(std::true_type{}) : go(std::false_type{});

@@ -38,7 +38,7 @@ struct WorkItem {
   int32_t t0;
   int32_t t1;
   int32_t part;
-  int32_t cost;  // planner's cost estimate; unused on the device
+  int32_t cost;  // planner's cost estimate (tiles x 64-column passes)
 };
 
 // Decode piece as the decode kernel reads it: every query row of sequence
@@ -132,6 +132,7 @@ struct AttnArgs {
   int page_shift;          // log2(page)
   float scale_log2;        // log2(e) / sqrt(128)
   float* part_scale;       // 8-bit caches: [slots][hq] powers of two that the partial rows are held under
+  int pair;                // 8-bit tile kernel: share b and b + pair are a compute unit's two (0: as listed)
   const float* scales;     // 8-bit caches: [16-token block][hkv][2] powers of two (kc, vc then hold e4m3 codes)
 };
 

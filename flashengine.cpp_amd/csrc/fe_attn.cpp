@@ -528,6 +528,7 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
     t.n_items = hdr + (mode ? kHdrTileEnd1 : kHdrTileEnd0);
     t.tile_off = reinterpret_cast<const int32_t*>(L.dev + L.lay.tshare[mode]);
     const int grid = L.graph ? L.grid_tile_cap : L.n_tshare[mode];
+    t.pair = !L.graph && !L.tile_cut[mode] && L.n_tshare[mode] > L.sh.num_cus ? L.sh.num_cus : 0;
     e = scales != nullptr ? launch_tile_kv8(t, L.bf16, causal != 0, L.tile_stream[mode], L.graph,
                                             L.tile_narrow[mode], L.tile_cut[mode] && L.sh.hkv % 2 == 0,
                                             std::max(grid, 1), st)

@@ -626,3 +626,133 @@ def test_cache_past_4_gib(dev):
         sb = W.Batch(hq=hq, hkv=hkv, page=16, blocks=6, starts=[n - rows], qlens=[rows], tables=[list(range(7))])
         W.build_metadata(sb)
         check_attention(sb, q, wk, wv, s, out.cpu(), lse.cpu(), True)
+
+
+# Batches whose lists take the paths that small ones do not: more than one
+# workgroup a compute unit, several items a workgroup, shares evened out.
+LISTS = [
+    # longest first, wide items, 512 shares of one to three items
+    (32, 8, [9, 100, 0, 31, 250, 77] * 2, [300, 201, 77, 128, 250, 33] * 2),
+    (16, 8, [7 * k % 90 for k in range(30)], [200 - 3 * k for k in range(30)]),
+    (64, 2, [11 * k % 400 for k in range(20)], [1 + 7 * k % 90 for k in range(20)]),
+    (6, 3, [7 * k % 50 for k in range(14)], [450 - 10 * k for k in range(14)]),
+    # narrow items, longest first (one kv head a workgroup)
+    (32, 8, [7 * k % 480 for k in range(70)], [16] * 70),
+    (24, 3, [13 * k % 470 for k in range(200)], [8] * 200),
+    # narrow items, equal cuts: pairs of kv heads, an odd count
+    (32, 8, [37 * k % 1500 + 300 for k in range(30)], [16] * 30),
+    (16, 2, [997, 3000, 40, 1800, 0, 512], [8, 5, 7, 8, 8, 8]),
+    (16, 4, [900] * 9, [9, 16, 12] * 3),
+    (24, 3, [2000, 900, 1711, 30], [8] * 4),
+    # equal cuts of wide items
+    (32, 8, [3000, 700, 12], [60, 33, 140]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", range(len(LISTS)))
+@pytest.mark.parametrize("causal", [True, False])
+def test_lists(dev, dtype, shape, causal):
+    hq, hkv, starts, qlens = LISTS[shape]
+    b, q, kc, vc, scales = case(hq, hkv, starts, qlens, 60 + shape, dtype)
+    out, lse, lists = attend(dev, b, q, kc, vc, scales, causal)
+    assert lists.tile_items > 0
+    if shape < 6:
+        assert lists.tile_items > 256 and lists.merge_rows == 0
+    check_attention(b, q, kc, vc, scales, out, lse, causal)
+    again, lse2, _ = attend(dev, b, q, kc, vc, scales, causal)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_shares_of_many_items(dev):
+    """More items a share than a wavefront has lanes: 34000 sequences of two
+    rows over the same three pages.  The first is right, the others are its bits."""
+    hq, hkv, n = 64, 1, 34000
+    one = W.Batch(hq=hq, hkv=hkv, page=16, blocks=4, starts=[38], qlens=[2], tables=[[2, 0, 3]])
+    W.build_metadata(one)
+    kc, vc, scales = cache(5, hkv, 3)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(2, hq, 128, generator=g).to(torch.bfloat16)
+    b = W.Batch(hq=hq, hkv=hkv, page=16, blocks=4, starts=[38] * n, qlens=[2] * n, tables=[[2, 0, 3]] * n)
+    W.build_metadata(b)
+    plan = feattn.Plan(hq, hkv, 128, 16, n, one.max_pages(), True, 4)
+    plan.prepare(b.qo, b.kv, b.pages, b.last, b.batch, b.rows)
+    assert plan.lists(True).tile_items == n
+    qd = q.to(dev).repeat(n, 1, 1)
+    out, lse = torch.zeros_like(qd), torch.zeros(2 * n, hq, device=dev)
+    plan.run_kv8(qd, kc.to(dev), vc.to(dev), scales.to(dev), out, lse=lse)
+    torch.cuda.synchronize()
+    plan.close()
+    check_attention(one, q, kc, vc, scales, out[:2].cpu(), lse[:2].cpu(), True)
+    assert (out.view(n, 2, hq, 128) == out[:2]).all() and (lse.view(n, 2, hq) == lse[:2]).all()
+
+
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [16, 16, 16], [70, 1, 20]])
+def test_without_lse(dev, qlens):
+    """No lse asked for: the same rows.  A batch without sequences writes nothing."""
+    b, q, kc, vc, scales = case(32, 8, [900, 30, 1500], qlens, 5)
+    want, _, _ = attend(dev, b, q, kc, vc, scales, True)
+    plan = feattn.Plan(32, 8, 128, 16, 3, b.max_pages(), True, b.blocks)
+    qd, kd, vd, sd = q.to(dev), kc.to(dev), vc.to(dev), scales.to(dev)
+    out = torch.full_like(qd, 7.0)
+    plan.prepare([0], [0], [], [], 0, 0)
+    plan.run_kv8(qd, kd, vd, sd, out)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    plan.prepare(b.qo, b.kv, b.pages, b.last, b.batch, b.rows)
+    plan.run_kv8(qd, kd, vd, sd, out)
+    torch.cuda.synchronize()
+    plan.close()
+    assert torch.equal(out.cpu(), want)
+
+
+def test_two_plans_on_two_streams(dev):
+    """Two plans' calls in flight at once, eager and as graphs, over caches of
+    their own: each has its own results."""
+    cases = [case(32, 8, [1500, 30, 700], [1, 1, 1], 5), case(32, 8, [1200, 64, 9], [40, 16, 130], 6)]
+    plans, tensors, graphs = [], [], []
+    for b, q, kc, vc, scales in cases:
+        plan = feattn.Plan(32, 8, 128, 16, 3, b.max_pages(), True, b.blocks)
+        plan.prepare(b.qo, b.kv, b.pages, b.last, b.batch, b.rows, graph=True)
+        t = [x.to(dev) for x in (q, kc, vc, scales)] + [torch.zeros_like(q, device=dev)]
+        lse = torch.zeros(b.rows, 32, device=dev)
+        plan.run_kv8(*t, lse=lse)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.run_kv8(*t, lse=lse)
+        plans.append(plan)
+        tensors.append((t, lse))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in cases]
+    for replay in (False, True):
+        for t, lse in tensors:
+            t[-1].zero_()
+            lse.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for plan, (t, lse), graph, st in zip(plans, tensors, graphs, streams):
+                with torch.cuda.stream(st):
+                    graph.replay() if replay else plan.run_kv8(*t, lse=lse)
+        torch.cuda.synchronize()
+        for (b, q, kc, vc, scales), (t, lse) in zip(cases, tensors):
+            check_attention(b, q, kc, vc, scales, t[-1].cpu(), lse.cpu(), True)
+    for plan in plans:
+        plan.close()
+
+
+def test_nothing_to_do(dev):
+    """No rows, or no kv heads and no queries: the calls return and write nothing."""
+    kc, vc, scales = (t.to(dev) for t in cache(2, 8, 1))
+    before = [t.clone() for t in (kc, vc, scales)]
+    x = torch.zeros(4, 8, 128, dtype=torch.bfloat16, device=dev)
+    slots = torch.zeros(4, dtype=torch.int64, device=dev)
+    table = W.rope_table(8, 1e4).to(dev)
+    for rows, hkv in ((0, 8), (4, 0)):
+        feattn.store_kv8(x, x, kc, vc, scales, slots, rows, hkv, 128, True, 32)
+        feattn.load_kv8(kc, vc, scales, slots, x, x, rows, hkv, 128, True, 32)
+    feattn.rope_append_kv8(x, x, x, kc, vc, scales, slots, slots, table, 0, 8, 8, 128, True, 8, 32)
+    torch.cuda.synchronize()
+    for t, w in zip((kc, vc, scales), before):
+        assert torch.equal(t, w)
+    assert not x.any()
