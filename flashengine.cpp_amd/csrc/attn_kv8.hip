@@ -190,11 +190,9 @@ __device__ __forceinline__ void put_combined(const AttnArgs& a, f32x4 acc, float
 // ===========================================================================
 // Decode
 // ===========================================================================
-// A wavefront owns a ring of U units in LDS, one stream of units per share:
-// per item its Q (16 columns x 256 bytes), then K and V of every 32 tokens
-// (4 KB of codes each).  A unit is five copies, four of 1 KB and one for its
-// scales (the two blocks' K or V scale; for a Q unit a filler, so that the
-// counts of copies in flight stay a multiple of five).
+// A wavefront owns a ring of U units in LDS, one stream of units per share: K
+// and V of every 32 tokens of its items (4 KB of codes each).  A unit is five
+// copies, four of 1 KB and one for its scales (the two blocks' K or V scale).
 //
 // Lane = 16*J + L.  Per 32 tokens:
 //   S^T = K Q^T: A = K rows (lane: token L, dims 16 (J + 4 s) .. +15 with one
@@ -204,14 +202,7 @@ __device__ __forceinline__ void put_combined(const AttnArgs& a, f32x4 acc, float
 constexpr int kKv8Unit = 4096;
 constexpr int kKv8Slot = kKv8Unit + 256;  // with the scales
 
-#ifndef FEATTN_KV8_UNITS
-#define FEATTN_KV8_UNITS 3
-#endif
-template <int WAVES>
-constexpr int kv8_units() {
-  static_assert(FEATTN_KV8_UNITS * WAVES * kKv8Slot <= kLdsBytes, "decode ring exceeds LDS");
-  return FEATTN_KV8_UNITS;
-}
+constexpr int kKv8Units = 2;  // 16 sequences of 32768 tokens 161 us, 163 with three; 64 of 512 to 4096 52.3, 52.9, 53.8 with four
 
 // ---- short-context items (see attn_short.hpp for the 16-bit form)
 constexpr int kShort8Wave = 16384;  // a wavefront's LDS: 64 tokens of V codes, then its 32 x 128 fp32 results
@@ -470,8 +461,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_short_kv8_kernel(AttnArgs 
 // prepares may plan the batch as short-context items.
 template <bool BF16, int WAVES, int NCB, bool ANY>
 __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kernel(AttnArgs a, int causal) {
-  constexpr int U = kv8_units<WAVES>();
-  static_assert(U >= 2, "the ring must hold one K/V pair");
+  constexpr int U = kKv8Units;
+  static_assert(U * WAVES * kKv8Slot <= kLdsBytes, "decode ring exceeds LDS");
   extern __shared__ __attribute__((aligned(16))) uint8_t dsm[];
   const int lane = threadIdx.x & 63;
   const int J = lane >> 4;
@@ -516,11 +507,9 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
   }
   // K operand: token L, chunk J + 4 s; Q operand for k-step 2 s + h: column L,
   // the 16-byte chunk of dims 16 (J + 4 s) + 8 h.
-  uint32_t k_lds[2], q_lds[4], v_lds[8];
+  uint32_t k_lds[2], v_lds[8];
 #pragma unroll
   for (int s = 0; s < 2; ++s) k_lds[s] = (uint32_t)(128 * L + 16 * ((J + 4 * s) ^ swz_k(L)));
-#pragma unroll
-  for (int k = 0; k < 4; ++k) q_lds[k] = (uint32_t)(256 * L + 16 * ((2 * (J + 4 * (k >> 1)) + (k & 1)) ^ L));
   v_operand_addr(J, L, v_lds);
 
   const size_t head_off = (size_t)kvh * kHeadDim;
@@ -533,16 +522,15 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
   };
 
   // ---- copy side: the next unit of the share's stream --------------------
-  // kind 0 = Q of item c_it, 1 = K / 2 = V of the 32 tokens at c_tok.  The
-  // following item (nw) and the next K unit's page ids are requested one item
-  // / one unit before they are needed.  A unit whose tokens end in its first
-  // block copies that one twice (what it brings is masked).
+  // K (c_key) or V of the 32 tokens at c_tok of item c_it.  The following item
+  // (nw) and the next K unit's page ids are requested one item / one unit
+  // before they are needed.  A unit whose tokens end in its first block copies
+  // that one twice (what it brings is masked).
   int c_it = it_begin;
   DecodeItem cw = rec.first;
   DecodeItem nw = cw;
   if (c_it + 1 < it_end) nw = ldc_ditem(a.ditems, c_it + 1);
-  int c_kind = 0;
-  int c_qb = 0;
+  bool c_key = true;
   int c_tok = cw.t0;
   int pg0 = rec.pg0;
   int pg1 = cw.t0 + 16 < cw.t1 ? rec.pg1 : rec.pg0;
@@ -563,23 +551,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
   };
   auto issue_one = [&]() {
     const uint32_t dst = ring + (uint32_t)(c_slot * kKv8Slot);
-    if (c_kind == 0) {
-      const int nc = cw.nq * G;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = 4 * r + J;
-        const int col = 16 * c_qb + n;
-        const int nn = col < nc ? col : 0;  // columns past the item repeat column 0
-        const int row = cw.q0 + nn / G;
-        const int head = kvh * G + nn % G;
-        lds_dma16(a.q + ((size_t)row * a.hq + head) * kHeadDim + 8 * (L ^ n), dst + 1024 * r);
-      }
-      lds_dma4(a.q, dst + kKv8Unit);
-      if (++c_qb == NCB) {
-        c_qb = 0;
-        c_kind = 1;
-      }
-    } else if (c_kind == 1) {
+    if (c_key) {
       blk0 = block_of(c_tok, pg0);
       blk1 = c_tok + 16 < cw.t1 ? block_of(c_tok + 16, pg1) : blk0;
       const uint32_t kg[4] = {k_goff[0], k_goff[1], k_goff[0], k_goff[1]};
@@ -592,23 +564,21 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
         pg0 = page_id(nw, nw.t0);
         pg1 = page_id(nw, min(nw.t0 + 16, nw.t1 - 1));
       }
-      c_kind = 2;
     } else {
       issue_codes(a.vc, v_goff, 1, dst);
       c_tok += 32;
-      c_kind = 1;
       if (c_tok >= cw.t1) {
         ++c_it;
         if (c_it < it_end) {
           cw = nw;
           c_tok = cw.t0;
-          c_kind = 0;
           if (c_it + 1 < it_end) nw = ldc_ditem(a.ditems, c_it + 1);
         } else {
           c_live = false;
         }
       }
     }
+    c_key = !c_key;
     ++issued;
     c_slot = c_slot + 1 == U ? 0 : c_slot + 1;
   };
@@ -627,7 +597,6 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
   typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 
   for (int it = it_begin; it < it_end; ++it) {
-    refill();
     const DecodeItem w = it == it_begin ? rec.first : ldc_ditem(a.ditems, it);
     const int t0 = w.t0;
     const int t1 = w.t1;
@@ -644,20 +613,20 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
       if (col_ok[cb]) lim[cb] = min(causal ? w.len - w.nq + (crow[cb] - w.q0) : w.len - 1, t1 - 1);
     }
 
+    // Q goes to registers: as units of the ring, in front of the item's K and V,
+    // it kept those from being asked for until it had come (two column blocks:
+    // 24 sequences of 5 rows 48.4 us, 47.6 so).
     u32x4 qf[NCB][4];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      if (cb > 0) refill();
-      wait_units<U, 5>(issued - consumed - 1);
-      const uint32_t qb = ring + (uint32_t)(r_slot * kKv8Slot);
+      const uint16_t* qp = a.q + ((size_t)crow[cb] * a.hq + chead[cb]) * kHeadDim + 16 * J;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        qf[cb][k] = lds_read16(qb + q_lds[k]);
+        qf[cb][k] = ld16(qp + 64 * (k >> 1) + 8 * (k & 1));
         if (!col_ok[cb]) qf[cb][k] = u32x4{0u, 0u, 0u, 0u};
       }
-      consumed += 1;
-      r_slot = r_slot + 1 == U ? 0 : r_slot + 1;
     }
+    refill();
 
     float m[NCB], lsum[NCB];
     f32x4 o[8][NCB];
@@ -723,6 +692,9 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
       u32x2 vw[8];
 #pragma unroll
       for (int db = 0; db < 8; ++db) vw[db] = lds_read_tr8(vst + v_lds[db]);
+      // With two column blocks V's slot is refilled at once (24 sequences of 5
+      // rows 46.2 us, 47.2 a step later); with one the wait costs more.
+      if constexpr (NCB > 1) refill_after_reads();
       __builtin_amdgcn_sched_barrier(0);
       u32x4 pf[NCB], pl[NCB];
       softmax_step<2, NCB>(sc, a.scale_log2, m, lsum, o, [&](int cb, const float (&x)[2][4]) {
@@ -738,7 +710,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) o[db][cb] = mfma16<BF16>(vf, pl[cb], o[db][cb]);
       }
-      consumed += 1;
+      if constexpr (NCB == 1) consumed += 1;
     }
 
 #pragma unroll
@@ -1008,7 +980,7 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
 // their reads meet in 256 bytes of a cache row.  One kv head's 128 bytes a row
 // are what such a stream reads alone, 5.8 TB/s with nothing computed against
 // 6.5 for two heads and 6.9 for four and more.
-constexpr int kBlk8Units = 3;
+constexpr int kBlk8Units = 2;  // (32 blocks of 16 rows over 2048 to 16384: 138.0 us, 140.4 with three)
 constexpr int kBlk8Wave = kBlk8Units * kKv8Slot;
 constexpr int kBlk8Head = kTile8Lds - 4 * kBlk8Wave;  // Q, or: exchange, then statistics
 constexpr int kBlk8Stats = 4 * 3 * 2048;  // what the wavefronts hand each other of 16 columns
@@ -1483,7 +1455,7 @@ template <bool BF16, int WAVES, int NCB, Decode8 KIND>
 static hipError_t decode8_launch(const AttnArgs& a, int causal, int grid, hipStream_t st) {
   void (*fn)(AttnArgs, int);
   size_t lds = 0;
-  if constexpr (KIND != Decode8::Short) lds = (size_t)WAVES * kv8_units<WAVES>() * kKv8Slot;
+  if constexpr (KIND != Decode8::Short) lds = (size_t)WAVES * kKv8Units * kKv8Slot;
   if constexpr (KIND != Decode8::Shares) lds = std::max(lds, short8_lds<WAVES>());
   if constexpr (KIND == Decode8::Short) fn = attn_short_kv8_kernel<BF16, WAVES, NCB>;
   else fn = attn_decode_kv8_kernel<BF16, WAVES, NCB, KIND == Decode8::Any>;
