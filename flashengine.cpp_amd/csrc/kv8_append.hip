@@ -202,10 +202,11 @@ __device__ __forceinline__ void key_row(u32x4 lo, u32x4 hi, const uint16_t* kw, 
     s += dpp64<kHalfMirror>(s);
     s = s * (1.0 / 128.0) + (double)eps;
     r = __builtin_amdgcn_rsq(s);  // good to some 2^-23: one step of Newton's iteration
-    r *= 1.5 - 0.5 * s * r * r;
+    if (s < __builtin_huge_val()) r *= 1.5 - 0.5 * s * r * r;
   }
   const float rf = (float)r;
-  uint32_t crossed = 0;
+  // (rows of a size whose fp32 factors would leave the normal range: in 64 bits)
+  uint32_t crossed = NORM && !(rf > 0x1p-100f && rf < 0x1p100f) ? 1u << 31 : 0u;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float a = in[e], b = in[8 + e];

@@ -188,8 +188,9 @@ int fe_attn_run_noalloc(const void* q, const void* k_cache, const void* v_cache,
 /* fe_attn_run on an 8-bit cache: the same plan, prepared the same way (one
  * prepare serves both kinds of cache), the same masks, rows and outputs.  Scores
  * and sums are exact products of 16-bit q and the cached values, accumulated in
- * fp32.  Slots outside the visible ranges are not used, whatever codes or
- * scales they hold. */
+ * fp32.  Slots that no row of their sequence sees are not used, whatever codes
+ * or scales they hold; a NaN in one that some rows see may reach the others, as
+ * in fe_attn_run. */
 int fe_attn_run_kv8(fe_attn_plan* plan, const void* q, const void* k_cache,
                     const void* v_cache, const float* scales, void* out,
                     float* lse, int causal, void* stream);

@@ -57,7 +57,7 @@ int fe_norm_rope_append(const void* qkv, int64_t row_stride, const void* q_weigh
 /* fe_norm_rope_append into an 8-bit cache (fe_attn.h: 8-bit caches): queries
  * and keys are normalized and rotated in fp32 and rounded once, the queries to
  * 16 bits, the keys to their codes (fe_norm_rope_append rounds to 16 bits
- * between the two steps as well). */
+ * between the two steps as well).  q_out must not overlap qkv. */
 int fe_norm_rope_append_kv8(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, float eps,
                             void* q_out, void* k_cache, void* v_cache, float* scales, const int64_t* pos,
                             const int64_t* slots, const float* cache, int rows, int hq, int hkv, int dim, int bf16,

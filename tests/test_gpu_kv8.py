@@ -241,6 +241,40 @@ def test_special_values(dev, dtype):
     assert torch.equal(torch.isnan(back), nan[:64]) and not torch.isinf(back).any()
 
 
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_norm_of_extreme_rows(dev, eps):
+    """Keys whose root mean square is near the ends of bf16's range, and one with
+    an infinity, whose norm leaves zeros and NaNs."""
+    hkv, rows, max_pos = 2, 48, 64
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(rows, 3 * hkv, 128, generator=g)
+    x[:16] *= 2.0 ** 125
+    x[16:32] *= 2.0 ** -126
+    x = x.to(torch.bfloat16)
+    x[40, 0, 3] = math.inf
+    x[41, 1, 70] = math.nan
+    assert torch.isfinite(x[:32]).all()
+    kw = (1 + 0.1 * torch.randn(128, generator=g)).to(torch.bfloat16)
+    kc, vc, scales = cache(4, hkv, 5)
+    kd, vd, sd = kc.to(dev), vc.to(dev), scales.to(dev)
+    pos, slots, table = torch.arange(rows), torch.arange(rows), W.rope_table(max_pos, 1e6)
+    qkv = x[:, hkv:].contiguous()
+    qkv[:, :hkv] = x[:, :hkv]
+    feattn.norm_rope_append_kv8(qkv.to(dev), 2 * hkv * 128, None, kw.to(dev), eps, None, kd, vd, sd, pos.to(dev),
+                                slots.to(dev), table.to(dev), rows, 0, hkv, True, max_pos, 64)
+    torch.cuda.synchronize()
+    want, size = kv8.norm_rope(qkv[:, :hkv], kw, eps, pos, table, max_pos)
+    nan = torch.isnan(want)
+    assert int(nan.sum()) == 2 + 128
+    _, s1 = kv8.append(kc, scales, 0, want, slots, torch.bfloat16)
+    assert torch.equal(sd.cpu()[:3, :, 0], s1[:3, :, 0])
+    got = kv8.load(kd.cpu(), s1, 0, slots)
+    assert torch.equal(torch.isnan(got), nan)
+    slack = 2.0 ** -18 * size
+    bound = half_step8(want.abs() + slack, s1[slots // 16][:, :, 0, None].double()) + slack
+    assert ((got - want).abs() <= bound)[~nan].all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("rows,hkv", [(1, 1), (33, 3), (700, 8)])
 def test_load(dev, dtype, rows, hkv):
