@@ -7,9 +7,16 @@
 // results are those of a 16-bit cache that holds the same values.
 //
 //  * attn_decode_kv8_kernel: a wavefront's share of the decode stream as in
-//    attn_decode_kernel, 32 tokens (two scale blocks) a step.
-//  * attn_short_kv8_kernel: short decode batches.
-//  * attn_tile_kv8_kernel: 64-token tiles shared by four wavefronts.
+//    attn_decode_kernel, 32 tokens (two scale blocks) a step.  HBM bound: 64
+//    sequences of 512 to 4096 tokens, 32/8 heads, 48.6 us, 290 MB at 6.0 TB/s
+//    (47.8 with nothing computed); 16 of 32768 6.7 TB/s.
+//  * attn_short_kv8_kernel: short decode batches; latency (4 of 512 tokens, 16/8
+//    heads, 8.0 us).
+//  * attn_tile_kv8_kernel: 64-token tiles shared by four wavefronts.  Bound by the
+//    overlap of conversion, softmax and MFMA: 2048 rows over 30000 tokens 932 us,
+//    1.12 PFLOP/s; 8192 prompt tokens 220 us, 0.86.
+//  * attn_block_kv8_kernel: items of at most 64 columns (32 draft blocks of 16 rows
+//    138 us, 4.7 TB/s and 0.59 PFLOP/s at once: issue of both, and HBM).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -752,12 +759,15 @@ struct Tile8Lanes {
   uint32_t k_lds[4], v_lds[8];
 };
 
-// Row of a block that a lane copies and converts in instruction u, and the
-// chunk positions (c ^ these) of row t in the 16-bit tile: rows t and t + 8, of
-// neighbouring groups of eight lanes, differ in the lowest bit, so that the
-// lanes' even (and odd) chunks of both meet no bank twice; the operand reads,
-// of 16 rows (K) and of eight consecutive ones (V), do not either.
-__device__ __forceinline__ int tile8_row(int lane, int u) { return 8 * ((lane >> 3) & 1) + (lane >> 4) + 4 * u; }
+// Row of a block and 16 codes of it that a lane copies and converts in
+// instruction u, and the chunk positions (c ^ these) of row t in the 16-bit tile.
+// A write of 16 bytes goes eight lanes at a time over 32 banks: four lanes with
+// the even (or odd) chunks of a half of row t and four with row t + 8's, whose
+// positions differ in the lowest bit, meet no bank twice (eight lanes of one row
+// did: 8 cycles more a write, 944 us against 932 for 2048 rows over 30000).  The operand reads, of 16 rows (K) and
+// of eight consecutive ones (V), do not either.
+__device__ __forceinline__ int tile8_row(int lane, int u) { return 8 * ((lane >> 2) & 1) + (lane >> 4) + 4 * u; }
+__device__ __forceinline__ int tile8_part(int lane) { return (lane & 3) | ((lane >> 1) & 4); }
 __device__ __forceinline__ int tile8_swz_k(int t) { return t ^ (t >> 3); }
 __device__ __forceinline__ int tile8_swz_v(int t) { return ((2 * t) & 15) | (t >> 3); }
 
@@ -766,7 +776,7 @@ __device__ __forceinline__ Tile8Lanes tile8_lanes(const AttnArgs& a, int lane) {
   const int row_bytes = a.hkv * kHeadDim;
   Tile8Lanes tl;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)(tile8_row(lane, r) * row_bytes + 16 * (lane & 7));
+  for (int r = 0; r < 2; ++r) tl.goff[r] = (uint32_t)(tile8_row(lane, r) * row_bytes + 16 * tile8_part(lane));
 #pragma unroll
   for (int s = 0; s < 4; ++s) tl.k_lds[s] = (uint32_t)(16 * (16 * L + ((4 * s + J) ^ tile8_swz_k(L))));
   const int k = L >> 2, m = L & 3, t = 4 * J + k;
@@ -920,7 +930,7 @@ __device__ __forceinline__ int tile8_item(const AttnArgs& a, const WorkItem& w, 
       // Rows at or past the item end become zero in V (0 * stale must stay 0).
       const uint32_t raw = lbase + (uint32_t)(kTile8Raw + wave * 4096);
       const int valid = t1 - (T + 16 * wave);
-      const int c = lane & 7;
+      const int c = tile8_part(lane);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int t = tile8_row(lane, u);

@@ -207,6 +207,29 @@ def test_token_by_token(dev, dtype):
         assert torch.equal(kd.cpu()[live], kc[live]) and torch.equal(vd.cpu()[live], vc[live]), t
 
 
+def test_rejected_drafts(dev):
+    """Runs of five written at positions that step back by what was rejected,
+    over block borders, the rejected rows large: live codes and all scales are
+    the oracle's."""
+    hkv, blocks, dt = 3, 4, torch.bfloat16
+    g = torch.Generator().manual_seed(15)
+    kc, vc, scales = cache(blocks, hkv, 3, dt)
+    kd, vd, sd = kc.to(dev), vc.to(dev), scales.to(dev)
+    at = 0
+    for accepted in (5, 2, 3, 1, 5, 1, 2, 4, 1, 1, 5, 3, 2):
+        k, v = (torch.randn(5, hkv, 128, generator=g) for _ in range(2))
+        k[accepted:] *= 64
+        k, v = k.to(dt), v.to(dt)
+        slots = torch.arange(at, at + 5)
+        kc, scales = kv8.append(kc, scales, 0, k.double(), slots, dt)
+        vc, scales = kv8.append(vc, scales, 1, v.double(), slots, dt)
+        feattn.store_kv8(k.to(dev), v.to(dev), kd, vd, sd, slots.to(dev), 5, hkv, 128, True, blocks * 16)
+        live = slice(0, at + 5)
+        assert torch.equal(sd.cpu(), scales), at
+        assert torch.equal(kd.cpu()[live], kc[live]) and torch.equal(vd.cpu()[live], vc[live]), at
+        at += accepted
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_special_values(dev, dtype):
     """NaN, infinities, the largest finite values, zeros and subnormals: the
