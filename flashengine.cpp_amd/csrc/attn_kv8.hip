@@ -13,8 +13,8 @@
 //  * attn_short_kv8_kernel: short decode batches; latency (4 of 512 tokens, 16/8
 //    heads, 8.0 us).
 //  * attn_tile_kv8_kernel: 64-token tiles shared by four wavefronts.  Bound by the
-//    overlap of conversion, softmax and MFMA: 2048 rows over 30000 tokens 932 us,
-//    1.12 PFLOP/s; 8192 prompt tokens 220 us, 0.86.
+//    overlap of conversion, softmax and MFMA: 2048 rows over 30000 tokens 925 us,
+//    1.13 PFLOP/s; 8192 prompt tokens 218 us, 0.87.
 //  * attn_block_kv8_kernel: items of at most 64 columns (32 draft blocks of 16 rows
 //    138 us, 4.7 TB/s and 0.59 PFLOP/s at once: issue of both, and HBM).
 #include <algorithm>
