@@ -721,6 +721,30 @@ def test_lists(dev, dtype, shape, causal):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+GROUPS = [
+    # head counts at the borders of the work units' columns
+    (33, 1, [70, 1000], [1, 2]),
+    (48, 1, [300, 40, 2000], [1, 1, 1]),
+    (96, 2, [1500, 20], [1, 3]),
+    (128, 1, [200, 900], [1, 2]),
+    (130, 2, [100, 700], [1, 1]),
+    (64, 2, [30, 800], [2, 4]),
+    (7, 7, [500, 20, 90], [1, 3, 40]),
+    (10, 5, [600, 33], [16, 70]),
+    (16, 16, [260, 1100], [1, 33]),
+]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", range(len(GROUPS)))
+def test_group_sizes(dev, shape, causal, graph):
+    hq, hkv, starts, qlens = GROUPS[shape]
+    b, q, kc, vc, scales = case(hq, hkv, starts, qlens, 80 + shape, "bf16")
+    out, lse, _ = attend(dev, b, q, kc, vc, scales, causal, graph=graph)
+    check_attention(b, q, kc, vc, scales, out, lse, causal)
+
+
 def test_shares_of_many_items(dev):
     """More items a share than a wavefront has lanes: 34000 sequences of two
     rows over the same three pages.  The first is right, the others are its bits."""
