@@ -33,6 +33,7 @@
 #include "attn_types.hpp"
 #include "device_util.hpp"
 #include "kernel_util.hpp"
+#include "kv8.hpp"
 
 namespace feattn {
 
@@ -732,12 +733,18 @@ __device__ __forceinline__ MergeRow ldc_merge(const MergeRow* rows, int i) {
   return MergeRow{ldc(p, 0), ldc(p, 1), ldc(p, 2), ldc(p, 3)};
 }
 
-template <bool BF16, bool SCALED, int BATCH>
+// Partial rows: in the attention's type; fp16 under a power of two of their own
+// (8-bit caches); the same with the remainders of their rounding (kv8.hpp).
+enum class PartRows { Plain, Scaled, ScaledLow };
+
+template <bool BF16, PartRows ROWS, int BATCH>
 __device__ __forceinline__ void merge_fold(const MergeArgs& a, const MergeRow& mr, int head, int d, int sp0,
                                            MergeState& s) {
   size_t slot[BATCH];
   float l[BATCH], f[BATCH];
   u32x2 rv[BATCH];  // four 16-bit partial values
+  constexpr bool SCALED = ROWS != PartRows::Plain, LOW = ROWS == PartRows::ScaledLow;
+  uint32_t lv[BATCH];  // LOW: their remainders
   // Past the last split the loads repeat it (a cache hit); what they brought
   // is replaced by zero with weight zero (a repeated infinity times zero would
   // be NaN).  A branch around each load lets the compiler move the 16-bit
@@ -756,6 +763,10 @@ __device__ __forceinline__ void merge_fold(const MergeArgs& a, const MergeRow& m
 #pragma unroll
   for (int u = 0; u < BATCH; ++u)
     rv[u] = *reinterpret_cast<const u32x2*>(a.part_o + slot[u] * kHeadDim + d);
+  if constexpr (LOW) {
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) lv[u] = *reinterpret_cast<const uint32_t*>(a.part_lo + slot[u] * kHeadDim + 8 * (d & 12) + (d >> 4) * 4);
+  }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int u = 0; u < BATCH; ++u)
@@ -774,7 +785,13 @@ __device__ __forceinline__ void merge_fold(const MergeArgs& a, const MergeRow& m
   for (int u = 0; u < BATCH; ++u) {
     rv[u] &= sp0 + u < mr.nsplit ? ~0u : 0u;
     constexpr bool B = BF16 && !SCALED;
-    const f32x4 v = {lo_f32<B>(rv[u][0]), hi_f32<B>(rv[u][0]), lo_f32<B>(rv[u][1]), hi_f32<B>(rv[u][1])};
+    f32x4 v = {lo_f32<B>(rv[u][0]), hi_f32<B>(rv[u][0]), lo_f32<B>(rv[u][1]), hi_f32<B>(rv[u][1])};
+    if constexpr (LOW) {
+      const int low = sp0 + u < mr.nsplit ? (int)lv[u] : 0;
+      const auto l0 = __builtin_amdgcn_cvt_pk_f32_fp8(low, false);
+      const auto l1 = __builtin_amdgcn_cvt_pk_f32_fp8(low, true);
+      v += f32x4{l0[0], l0[1], l1[0], l1[1]} * (1.f / kPartLo);
+    }
     s.wsum += l[u];
     s.acc += (SCALED ? l[u] * f[u] : l[u]) * v;
   }
@@ -794,9 +811,7 @@ __device__ __forceinline__ void merge_write(const MergeArgs& a, int row, int hea
 // header names; an eager launch is handed the list and its length.
 enum class MergeForm { Narrow, Wide, Header };
 
-// SCALED: rows of the 8-bit caches' kernels, fp16 under a power of two of their
-// own (part_store, kv8.hpp).
-template <bool BF16, MergeForm FORM, bool SCALED>
+template <bool BF16, MergeForm FORM, PartRows ROWS>
 __global__ __launch_bounds__(256) void attn_merge_kernel(MergeArgs a) {
   constexpr int WAVES = 4, kFew = 4, kNarrow = 8, kWide = 16;
   const int lane = threadIdx.x & 63;
@@ -819,9 +834,9 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(MergeArgs a) {
       const int hh = h < a.hq ? h : a.hq - 1;
       MergeState s{kNegInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
       if (mr.nsplit <= kFew) {
-        merge_fold<BF16, SCALED, kFew>(a, mr, hh, d, 0, s);
+        merge_fold<BF16, ROWS, kFew>(a, mr, hh, d, 0, s);
       } else {
-        for (int sp0 = 0; sp0 < mr.nsplit; sp0 += kNarrow) merge_fold<BF16, SCALED, kNarrow>(a, mr, hh, d, sp0, s);
+        for (int sp0 = 0; sp0 < mr.nsplit; sp0 += kNarrow) merge_fold<BF16, ROWS, kNarrow>(a, mr, hh, d, sp0, s);
       }
       if (h < a.hq) merge_write<BF16>(a, mr.row, h, d, s);
     }
@@ -835,7 +850,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(MergeArgs a) {
     const int h = 2 * (pair % hpairs) + (lane >> 5);
     MergeState s{kNegInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
     for (int sp0 = kWide * wave; sp0 < mr.nsplit; sp0 += kWide * WAVES)
-      merge_fold<BF16, SCALED, kWide>(a, mr, h < a.hq ? h : a.hq - 1, d, sp0, s);
+      merge_fold<BF16, ROWS, kWide>(a, mr, h < a.hq ? h : a.hq - 1, d, sp0, s);
     sh_acc[wave][lane] = s.acc;
     if (d == 0) {
       sh_m[wave][lane >> 5] = s.m;
@@ -958,19 +973,25 @@ hipError_t launch_stage_copy(void* dst, const void* src, size_t bytes, hipStream
   return hipGetLastError();
 }
 
-template <bool BF16, bool SCALED>
+template <bool BF16, PartRows ROWS>
 static void merge_launch(const MergeArgs& a, int grid, hipStream_t st) {
   if (a.count_base != nullptr)
-    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Header, SCALED>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Header, ROWS>), dim3(grid), dim3(256), 0, st, a);
   else if (a.wide)
-    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Wide, SCALED>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Wide, ROWS>), dim3(grid), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Narrow, SCALED>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_merge_kernel<BF16, MergeForm::Narrow, ROWS>), dim3(grid), dim3(256), 0, st, a);
 }
 
 hipError_t launch_merge(const MergeArgs& a, bool bf16, int grid, hipStream_t st) {
-  if (a.part_scale != nullptr) bf16 ? merge_launch<true, true>(a, grid, st) : merge_launch<false, true>(a, grid, st);
-  else bf16 ? merge_launch<true, false>(a, grid, st) : merge_launch<false, false>(a, grid, st);
+  if (a.part_scale == nullptr) {
+    bf16 ? merge_launch<true, PartRows::Plain>(a, grid, st) : merge_launch<false, PartRows::Plain>(a, grid, st);
+  } else if (bf16) {
+    merge_launch<true, PartRows::Scaled>(a, grid, st);
+  } else {
+    a.part_lo != nullptr ? merge_launch<false, PartRows::ScaledLow>(a, grid, st)
+                         : merge_launch<false, PartRows::Scaled>(a, grid, st);
+  }
   return hipGetLastError();
 }
 

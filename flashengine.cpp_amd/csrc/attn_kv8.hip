@@ -99,8 +99,9 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[P][NCB], float scale, f
 
 // Probabilities as two 16-bit operands whose sum they are within 2^-17 (bf16) or
 // 2^-23 (fp16): hi rounded, lo the rest.  The decode kernels wait for memory,
-// not for the MFMA, so the second product costs them nothing, and their results
-// carry the output's rounding alone (with hi only the error was 1.4 times that).
+// not for the MFMA, so the second product costs them nothing (two column blocks:
+// 1.1 us of 46.4), and their results carry the output's rounding alone (with hi
+// only the error was 1.4 times that).
 template <bool BF16>
 __device__ __forceinline__ void pack2_split(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pack2<BF16>(a, b);
@@ -129,6 +130,18 @@ __device__ __forceinline__ void v_operand_addr(int J, int L, uint32_t (&v_lds)[8
   for (int db = 0; db < 8; ++db) v_lds[db] = (uint32_t)(128 * t + 16 * (db ^ swz_v(t)) + 8 * m);
 }
 
+// Four values of a partial row, already under its scale, to element `at`; the
+// codes of what their rounding leaves are returned for part_lo, where a row has
+// dims 16 db + 4 J .. + 3 at byte 32 J + 4 db: a column's lane stores 32 bytes.
+template <bool BF16>
+__device__ __forceinline__ uint32_t put_part(const AttnArgs& a, size_t at, f32x4 v) {
+  const u32x2 hi = {pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])};
+  *reinterpret_cast<u32x2*>(a.part_o + at) = hi;
+  if constexpr (BF16) return 0u;
+  v = (v - f32x4{lo_f32<false>(hi[0]), hi_f32<false>(hi[0]), lo_f32<false>(hi[1]), hi_f32<false>(hi[1])}) * kPartLo;
+  return kv8_encode4(v[0], v[1], v[2], v[3]);
+}
+
 // A column's results (lane 16 J + L: dims 16 db + 4 J + r): to `out` and `lse`,
 // or to partial row `slot` when the row is split.
 template <bool BF16>
@@ -155,11 +168,15 @@ __device__ __forceinline__ void put_column(const AttnArgs& a, const f32x4 (&o)[8
   float is;
   const float sc = part_scale_of(mx, is);
   const size_t oi = (size_t)slot * a.hq + head;
-  uint16_t* op = a.part_o + oi * kHeadDim + 4 * J;
+  u32x4 low[2];
 #pragma unroll
   for (int db = 0; db < 8; ++db)
-    *reinterpret_cast<u32x2*>(op + 16 * db) = u32x2{pack2<false>(o[db][0] * inv * is, o[db][1] * inv * is),
-                                                    pack2<false>(o[db][2] * inv * is, o[db][3] * inv * is)};
+    low[db >> 2][db & 3] = put_part<BF16>(a, oi * kHeadDim + 4 * J + 16 * db, o[db] * inv * is);
+  if (!BF16 && a.part_lo != nullptr) {
+    u32x4* to = reinterpret_cast<u32x4*>(a.part_lo + oi * kHeadDim + 32 * J);
+    to[0] = low[0];
+    to[1] = low[1];
+  }
   if (J == 0) {
     a.part_lse[oi] = l2;
     a.part_scale[oi] = sc;
@@ -186,8 +203,9 @@ __device__ __forceinline__ void put_combined(const AttnArgs& a, f32x4 acc, float
   float is;
   const float sc = part_scale_of(mx, is);
   const size_t oi = (size_t)slot * a.hq + head;
-  *reinterpret_cast<u32x2*>(a.part_o + oi * kHeadDim + 4 * c) =
-      u32x2{pack2<false>(acc[0] * is, acc[1] * is), pack2<false>(acc[2] * is, acc[3] * is)};
+  const uint32_t low = put_part<BF16>(a, oi * kHeadDim + 4 * c, acc * is);
+  if (!BF16 && a.part_lo != nullptr)
+    *reinterpret_cast<uint32_t*>(a.part_lo + oi * kHeadDim + 32 * (c & 3) + 4 * (c >> 2)) = low;
   if (c == 0) {
     a.part_lse[oi] = l2;
     a.part_scale[oi] = sc;
@@ -1317,10 +1335,12 @@ __device__ __forceinline__ void block8_items(const AttnArgs& a, int it0, int it1
             float is;
             const float sc = part_scale_of(bound * inv, is);
             const size_t oi = (size_t)(w.part + r) * a.hq + head;
+            u32x2 low;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              *reinterpret_cast<u32x2*>(a.part_o + oi * kHeadDim + 32 * wv + 16 * i + 4 * Jc) =
-                  u32x2{pack2<false>(acc[i][0] * is, acc[i][1] * is), pack2<false>(acc[i][2] * is, acc[i][3] * is)};
+              low[i] = put_part<BF16>(a, oi * kHeadDim + 32 * wv + 16 * i + 4 * Jc, acc[i] * is);
+            if (!BF16 && a.part_lo != nullptr)
+              *reinterpret_cast<u32x2*>(a.part_lo + oi * kHeadDim + 32 * Jc + 8 * wv) = low;
             if (wv == 0 && Jc == 0) {
               a.part_lse[oi] = l2;
               a.part_scale[oi] = sc;

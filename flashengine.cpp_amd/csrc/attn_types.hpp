@@ -132,6 +132,7 @@ struct AttnArgs {
   int page_shift;          // log2(page)
   float scale_log2;        // log2(e) / sqrt(128)
   float* part_scale;       // 8-bit caches: [slots][hq] powers of two that the partial rows are held under
+  uint8_t* part_lo;        // 8-bit caches, fp16 calls with tiles: [slots][hq][128], what those rows' rounding left
   int pair;                // 8-bit tile kernel: share b and b + pair are a compute unit's two (0: as listed)
   const float* scales;     // 8-bit caches: [16-token block][hkv][2] powers of two (kc, vc then hold e4m3 codes)
 };
@@ -146,6 +147,7 @@ struct MergeArgs {
   const uint16_t* part_o;
   const float* part_lse;
   const float* part_scale;    // null: rows in the attention's type; else fp16 rows, to be scaled by these
+  const uint8_t* part_lo;     // with part_scale, or null: what those rows' rounding left
   int hq;
 };
 

@@ -327,6 +327,7 @@ struct Launch {
   uint16_t* part_o = nullptr;    // 16-bit split-KV partial rows
   float* part_lse = nullptr;
   float* part_scale = nullptr;   // the partial rows' powers of two (8-bit caches)
+  uint8_t* part_lo = nullptr;    // fp16: the partial rows' remainders (8-bit caches)
   bool bf16 = true;
   bool graph = false;
   int graph_tile = -1;  // graph plans: the first graph prepare had tile work (1) or not (0)
@@ -506,6 +507,9 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
   a.scale_log2 = 1.4426950408889634f / 11.313708498984761f;  // log2(e) / sqrt(128)
   a.scales = scales;
   a.part_scale = L.part_scale;
+  // (decode kernels alone have one rounding less and need no remainders)
+  const bool low = scales != nullptr && !L.bf16 && (L.graph ? L.graph_tile > 0 : L.n_tile[mode] > 0);
+  a.part_lo = low ? L.part_lo : nullptr;
   hipError_t e;
   if (L.graph || L.n_decode > 0 || L.n_short > 0) {
     AttnArgs d = a;
@@ -549,6 +553,7 @@ int launch_all(const Launch& L, const void* q, const void* k_cache, const void* 
     m.part_o = L.part_o;
     m.part_lse = L.part_lse;
     m.part_scale = scales != nullptr ? L.part_scale : nullptr;
+    m.part_lo = a.part_lo;
     m.hq = L.sh.hq;
     m.wide = L.wide_merge[mode] ? 1 : 0;
     e = launch_merge(m, L.bf16, merge_grid(L, mode), st);
@@ -707,7 +712,9 @@ int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int m
   if (hipHostGetDevicePointer(reinterpret_cast<void**>(&p->host_dev), p->host, 0) != hipSuccess ||
       p->host_dev == nullptr)
     return cleanup(FE_EDEVICE, "hipHostGetDevicePointer(plan staging) failed");
-  if (hipMalloc(&p->part_o, (size_t)sh.partial_cap * hq * kHeadDim * sizeof(uint16_t)) != hipSuccess)
+  // the partial rows, and behind fp16 ones a byte each of their remainders (8-bit caches)
+  const size_t part_elems = (size_t)sh.partial_cap * hq * kHeadDim;
+  if (hipMalloc(&p->part_o, part_elems * (bf16 ? 2 : 3)) != hipSuccess)
     return cleanup(FE_ENOMEM, "hipMalloc(split-KV partials) failed");
   // the log-sum-exps, and behind them the rows' scales (8-bit caches)
   if (hipMalloc(&p->part_lse, 2 * (size_t)sh.partial_cap * hq * sizeof(float)) != hipSuccess)
@@ -720,6 +727,7 @@ int fe_attn_plan_create(int hq, int hkv, int dim, int page, int max_batch, int m
   p->run.dev = p->dev;
   p->run.part_o = p->part_o;
   p->run.part_lse = p->part_lse;
+  if (!bf16) p->run.part_lo = reinterpret_cast<uint8_t*>(p->part_o + part_elems);
   p->run.part_scale = p->part_lse + (size_t)sh.partial_cap * hq;
   *plan_out = p;
   return FE_OK;

@@ -54,10 +54,17 @@ __device__ __forceinline__ u32x4 kv8_decode8(uint32_t w0, uint32_t w1, float s0,
 }
 
 // Split-KV partial rows of these kernels: fp16 under a power of two of the
-// row's own, four bits more than a bf16 row at the same size (with bf16 rows
-// the error of split results was 1.7 times that of rounding them once, 1.4
-// with these, as for rows that are not split).  mx: the row's largest
-// magnitude; returns the scale s with mx in [s, 2 s), and its inverse.
+// row's own, three bits more than a bf16 row at the same size.  For fp16 results
+// of tiles, whose probabilities are rounded as well, that would be a third
+// rounding (1.7 times the error of the output's alone, 1.4 without it): there the
+// remainder of each value, at most 2^-11 of the scale, goes along as an e4m3 code
+// in units of 2^-19.  (Calls
+// without tiles have none: their probabilities have two parts, and 24 sequences
+// of 5 rows took 52.3 us with remainders and one part, 46.4 so.  32 draft blocks
+// take 143 us with them, 139 without.)
+// mx: the row's largest magnitude; returns the scale s with mx in [s, 2 s), and
+// its inverse.
+constexpr float kPartLo = 0x1p19f;
 __device__ __forceinline__ float part_scale_of(float mx, float& inverse) {
   const uint32_t s = min(max(__float_as_uint(mx) & kInfBits, 1u << 23), 253u << 23);
   inverse = __uint_as_float((254u << 23) - s);

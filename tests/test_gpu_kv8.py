@@ -721,6 +721,23 @@ def test_lists(dev, dtype, shape, causal):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("starts,qlens", [([3000, 5000, 1200, 4000], [16] * 4), ([9000, 4000], [60, 70]),
+                                          ([4000, 7000, 9000, 2500], [1, 1, 5, 1])])
+def test_split_rows_in_fp16(dev, starts, qlens):
+    """fp16 rows split over several work units carry two roundings of their size,
+    as unsplit ones do: 2^0.5 times the output's alone in the mean square (three
+    would be 1.73), over 10^5 values and more to within a few per cent."""
+    b, q, kc, vc, scales = case(32, 8, starts, qlens, 91, "f16")
+    out, lse, lists = attend(dev, b, q, kc, vc, scales, False)
+    assert lists.merge_rows == b.rows
+    check_attention(b, q, kc, vc, scales, out, lse, False)
+    at = torch.arange(kc.shape[0])
+    want = kv8.attention(b, q, kv8.load(kc, scales, 0, at), kv8.load(vc, scales, 1, at), False)[0]
+    err = (out.double() - want).square().mean().sqrt()
+    rounding = (want.half().double() - want).square().mean().sqrt()
+    assert err <= 1.55 * rounding, (err / rounding).item()
+
+
 GROUPS = [
     # head counts at the borders of the work units' columns
     (33, 1, [70, 1000], [1, 2]),
