@@ -570,7 +570,7 @@ __global__ __launch_bounds__(64 * WAVES, ANY ? 2 : 1) void attn_decode_kv8_kerne
     lds_dma16<true>(b0, goff[0], dst);
     lds_dma16<true>(b0, goff[1], dst + 1024);
     lds_dma16<true>(b1, goff[2], dst + 2048);
-    lds_dma16<true>(b1, goff[3], dst + 3072);
+    lds_dma16<true>(b1, goff[3], dst + 3 * 1024);
     const size_t at = (lane & 1) ? blk1 : blk0;
     lds_dma4(a.scales + 2 * (at * (size_t)a.hkv + (size_t)kvh) + side, dst + kKv8Unit);
   };
@@ -1081,7 +1081,7 @@ __device__ __forceinline__ void block8_items(const AttnArgs& a, int it0, int it1
     lds_dma16<STREAM>(b0, goff[0], dst);
     lds_dma16<STREAM>(b0, goff[1], dst + 1024);
     lds_dma16<STREAM>(b1, goff[2], dst + 2048);
-    lds_dma16<STREAM>(b1, goff[3], dst + 3072);
+    lds_dma16<STREAM>(b1, goff[3], dst + 3 * 1024);
     const size_t at = (lane & 1) ? blk1 : blk0;
     lds_dma4(a.scales + 2 * (at * (size_t)a.hkv + (size_t)c_kvh) + side, dst + kKv8Unit);
   };
